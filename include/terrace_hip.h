@@ -489,6 +489,79 @@ TERRACE_API int terrace_dispatch(const void *x, const int64_t *expert_idx, const
                                  void *permuted, void *planes, const int64_t *plane_offsets, void *workspace,
                                  size_t workspace_bytes, terrace_stream_t stream);
 
+/* ---- around the experts of one block ----
+ * No counterpart in the reference, which leaves the experts, the gradient of the weighted combine and the norms to the
+ * layer around it.  As everywhere here: device pointers, the caller's workspace and stream, nothing allocated, kept or
+ * thrown.  `rows in expert order` and tokens_per_expert are what terrace_regroup / terrace_hopb_scatter and
+ * terrace_expert_sort leave: the rows of expert 0, then those of expert 1, and so on. */
+
+/* Tokens to expert order without the hops between.  expert_idx [T,k] i64; an id below 0 is a pair without an expert here
+ * (another rank's, or masked), an id >= n_experts is one too and sets TERRACE_FAULT_ID_RANGE.  The P = T*k pairs are
+ * placed in stable order of expert: where [T,k] i64 is the place of each pair (-1: no expert), tokens_per_expert
+ * [n_experts] i64, offsets [n_experts + 1] i64 their exclusive prefix (the last entry: pairs with an expert).
+ *   x [T,row_bytes] (NULL with rows NULL: the index planes only) -> rows [P,row_bytes], rows[where[t,j]] = x[t]; rows
+ * from offsets[n_experts] on are zeros.  n_experts <= 2048.  status may be NULL. */
+TERRACE_API size_t terrace_expert_sort_workspace(int64_t T, int k, int n_experts);
+TERRACE_API int terrace_expert_sort(const void *x, const int64_t *expert_idx, int64_t T, int64_t row_bytes, int k,
+                                    int n_experts, void *rows, int64_t *where, int64_t *tokens_per_expert,
+                                    int64_t *offsets, int32_t *status, void *workspace, size_t workspace_bytes,
+                                    terrace_stream_t stream);
+
+/* The gradient of the weighted way back y[t] = sum_j weights[t,j] * rows[where[t,j]] (terrace_combine over the plan of
+ * terrace_expert_sort, in which a place belongs to at most one pair):
+ *   d_rows[where[t,j]] = weights[t,j] * dy[t];   d_weights[t,j] = <dy[t], rows[where[t,j]]>  (0 where there is no expert)
+ * in fp32, each rounded once.  rows and d_rows [n_rows,hidden] of row_dtype, dy [T,hidden] of dy_dtype, weights and
+ * d_weights [T,k] of w_dtype (F32, BF16, F16); weights NULL: all ones.  d_rows or d_weights may be NULL (not wanted;
+ * rows is read for d_weights only).  Rows of d_rows from *n_live on (offsets[n_experts] of the plan, device memory)
+ * are written as zeros. */
+TERRACE_API int terrace_expert_unsort_grad(const void *rows, int row_dtype, const void *dy, int dy_dtype,
+                                           const int64_t *where, const void *weights, int w_dtype, int64_t T, int k,
+                                           int64_t hidden, int64_t n_rows, const int64_t *n_live, void *d_rows,
+                                           void *d_weights, terrace_stream_t stream);
+
+/* 4-bit expert weights.  codes [n_experts,N,K/2] bytes (k even in the low nibble), scales [n_experts,N,K/group] 16-bit
+ * floats, zeros [n_experts,N,K/group] bytes 0..15 or NULL (8 everywhere): weight = scale * (code - zero).  group is 32, 64
+ * or 128 and divides K.  terrace_w4_pack lays them out for terrace_w4_linear, once per weight; terrace_w4_packed_bytes
+ * tells the size of each packed plane (what: 0 codes, 1 scales, 2 zeros; 0 bytes: a shape that is not taken). */
+TERRACE_API size_t terrace_w4_packed_bytes(int n_experts, int64_t N, int64_t K, int group, int what);
+TERRACE_API int terrace_w4_pack(const void *codes, const void *scales, const void *zeros, int n_experts, int64_t N,
+                                int64_t K, int group, void *packed_codes, void *packed_scales, void *packed_zeros,
+                                terrace_stream_t stream);
+
+/* out[i] = W[e] x[i] for the rows i of expert e: x [P,K] and out [P,N] of dtype (BF16 or F16, the scales' type too),
+ * rows in expert order, tokens_per_expert [n_experts] i64 (NULL with one expert: all rows are its rows).  swiglu != 0: N is even and out [P,N/2] =
+ * silu(first half of the columns) * second half, taken before the one rounding.  Sums are fp32.  Rows past the last
+ * expert's are written as zeros.  Counts below 0 are taken as 0, and none reaches past row P.  x and the packed codes on 16 bytes.
+ * Made for few rows per expert (every 16, 32 or 64 rows read the expert's weights once). */
+TERRACE_API int terrace_w4_linear(const void *x, int dtype, int64_t P, const int64_t *tokens_per_expert,
+                                  const void *packed_codes, const void *packed_scales, const void *packed_zeros,
+                                  int n_experts, int64_t N, int64_t K, int group, int swiglu, void *out,
+                                  terrace_stream_t stream);
+
+/* Between two blocks: h = residual + scale * gate * p with p = y / rms(y) * w_post, and n = h / rms(h) * w_pre, where
+ * rms(v) = sqrt(mean(v^2) + eps), in fp32 with one rounding per output (n from the unrounded h).
+ *   y [T,H] of y_dtype and residual [T,H] of r_dtype (y_dtype or F32); h [T,H] of r_dtype, n [T,H] of y_dtype.
+ *   w_post [H] (NULL: p = y), gate [H] or [T] by gate_kind (NULL with TERRACE_GATE_NONE), w_pre [H] (NULL: no n).
+ *   y NULL (with w_post and gate NULL): only the norm before a block, h = residual (h may then be NULL).
+ *   stats [T,2] f32 (may be NULL): 1/rms of y and of h, for terrace_block_norm_grad.
+ * H up to 16384 where it is a multiple of 8 and every row and weight lies on 16 bytes, up to 8192 otherwise. */
+enum terrace_gate_kind { TERRACE_GATE_NONE = 0, TERRACE_GATE_CHANNEL = 1, TERRACE_GATE_TOKEN = 2 };
+TERRACE_API int terrace_block_norm(const void *y, int y_dtype, const void *residual, int r_dtype, const void *w_post,
+                                   int post_dtype, const void *gate, int gate_dtype, int gate_kind, const void *w_pre,
+                                   int pre_dtype, float scale, float eps, int64_t T, int64_t H, void *h, void *n,
+                                   float *stats, terrace_stream_t stream);
+
+/* Its gradient, from the same inputs, the saved stats and the gradients dh [T,H] of r_dtype and dn [T,H] of y_dtype
+ * (either NULL: zero).  dy of y_dtype, d_residual of r_dtype, d_post / d_gate / d_pre of their vectors' dtypes and
+ * shapes; any may be NULL.  Sums over the rows are added in a fixed order. */
+TERRACE_API size_t terrace_block_norm_grad_workspace(int64_t T, int64_t H);
+TERRACE_API int terrace_block_norm_grad(const void *y, int y_dtype, const void *residual, int r_dtype,
+                                        const void *w_post, int post_dtype, const void *gate, int gate_dtype,
+                                        int gate_kind, const void *w_pre, int pre_dtype, float scale, float eps,
+                                        int64_t T, int64_t H, const float *stats, const void *dh, const void *dn,
+                                        void *dy, void *d_residual, void *d_post, void *d_gate, void *d_pre,
+                                        void *workspace, size_t workspace_bytes, terrace_stream_t stream);
+
 /* ---- the entry point that brings its own scratch memory ----
  * No counterpart in the reference.  It is for callers that cannot allocate device memory at all -- code under
  * HIP graph capture, serving loops that must stay off the allocator, harnesses that forbid hipMalloc -- and so

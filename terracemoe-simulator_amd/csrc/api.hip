@@ -99,6 +99,28 @@ int run_k1_arrival_move(const void *rx, int64_t R, int64_t row_bytes, int quota,
                         const void *ws, size_t ws_bytes, hipStream_t s);
 int run_regroup_move(const void *node_rx, int64_t P, int64_t row_bytes, int epr, int64_t capacity, void *permuted,
                      const void *ws, size_t ws_bytes, hipStream_t s);
+size_t expert_sort_workspace(int64_t T, int k, int n_experts);
+int run_expert_sort(const void *x, const int64_t *expert_idx, int64_t T, int64_t row_bytes, int k, int n_experts,
+                    void *rows, int64_t *where, int64_t *tokens_per_expert, int64_t *offsets, int32_t *status, void *ws,
+                    size_t ws_bytes, hipStream_t s);
+int run_expert_unsort_grad(const void *src, int src_dtype, const void *dy, int dy_dtype, const int64_t *where,
+                           const void *weights, int w_dtype, int64_t T, int k, int64_t hidden, int64_t n_rows,
+                           const int64_t *live, void *d_rows, void *d_weights, hipStream_t s);
+size_t w4_packed_bytes(int n_experts, int64_t N, int64_t K, int group, int what);
+int run_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int n_experts, int64_t N, int64_t K,
+                int group, void *packed_codes, void *packed_scales, void *packed_zeros, hipStream_t s);
+int run_w4_linear(const void *x, int dtype, int64_t P, const int64_t *counts, const void *codes, const void *scales,
+                  const void *zeros, int n_experts, int64_t N, int64_t K, int group, int swiglu, void *out,
+                  hipStream_t s);
+int run_block_norm(const void *y, int y_dtype, const void *residual, int r_dtype, const void *w_post, int post_dtype,
+                   const void *gate, int gate_dtype, int gate_kind, const void *w_pre, int pre_dtype, float scale,
+                   float eps, int64_t T, int64_t H, void *h, void *n, float *stats, hipStream_t s);
+size_t block_norm_grad_workspace(int64_t T, int64_t H);
+int run_block_norm_grad(const void *y, int y_dtype, const void *residual, int r_dtype, const void *w_post,
+                        int post_dtype, const void *gate, int gate_dtype, int gate_kind, const void *w_pre,
+                        int pre_dtype, float scale, float eps, int64_t T, int64_t H, const float *stats, const void *dh,
+                        const void *dn, void *dy, void *d_residual, void *d_post, void *d_gate, void *d_pre, void *ws,
+                        size_t ws_bytes, hipStream_t s);
 }  // namespace terrace
 
 using namespace terrace;
@@ -531,6 +553,58 @@ int terrace_hopa_send_splits(const int64_t *node_counts, int world, int rpn, int
     if (world <= 0 || rpn <= 0 || world % rpn || my_local < 0 || my_local >= rpn || !node_counts || !send)
         return TERRACE_EINVAL;
     return launch_send_splits(node_counts, world, rpn, my_local, send, (hipStream_t)stream);
+}
+
+size_t terrace_expert_sort_workspace(int64_t T, int k, int n_experts) { return expert_sort_workspace(T, k, n_experts); }
+
+int terrace_expert_sort(const void *x, const int64_t *expert_idx, int64_t T, int64_t row_bytes, int k, int n_experts,
+                        void *rows, int64_t *where, int64_t *tokens_per_expert, int64_t *offsets, int32_t *status,
+                        void *workspace, size_t workspace_bytes, terrace_stream_t stream) {
+    return run_expert_sort(x, expert_idx, T, row_bytes, k, n_experts, rows, where, tokens_per_expert, offsets, status,
+                           workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int terrace_expert_unsort_grad(const void *rows, int row_dtype, const void *dy, int dy_dtype, const int64_t *where,
+                               const void *weights, int w_dtype, int64_t T, int k, int64_t hidden, int64_t n_rows,
+                               const int64_t *n_live, void *d_rows, void *d_weights, terrace_stream_t stream) {
+    return run_expert_unsort_grad(rows, row_dtype, dy, dy_dtype, where, weights, w_dtype, T, k, hidden, n_rows, n_live,
+                                  d_rows, d_weights, (hipStream_t)stream);
+}
+
+size_t terrace_w4_packed_bytes(int n_experts, int64_t N, int64_t K, int group, int what) {
+    return what < 0 || what > 2 ? 0 : w4_packed_bytes(n_experts, N, K, group, what);
+}
+
+int terrace_w4_pack(const void *codes, const void *scales, const void *zeros, int n_experts, int64_t N, int64_t K,
+                    int group, void *packed_codes, void *packed_scales, void *packed_zeros, terrace_stream_t stream) {
+    return run_w4_pack((const uint8_t *)codes, scales, (const uint8_t *)zeros, n_experts, N, K, group, packed_codes,
+                       packed_scales, packed_zeros, (hipStream_t)stream);
+}
+
+int terrace_w4_linear(const void *x, int dtype, int64_t P, const int64_t *tokens_per_expert, const void *packed_codes,
+                      const void *packed_scales, const void *packed_zeros, int n_experts, int64_t N, int64_t K, int group,
+                      int swiglu, void *out, terrace_stream_t stream) {
+    return run_w4_linear(x, dtype, P, tokens_per_expert, packed_codes, packed_scales, packed_zeros, n_experts, N, K, group,
+                         swiglu, out, (hipStream_t)stream);
+}
+
+int terrace_block_norm(const void *y, int y_dtype, const void *residual, int r_dtype, const void *w_post, int post_dtype,
+                       const void *gate, int gate_dtype, int gate_kind, const void *w_pre, int pre_dtype, float scale,
+                       float eps, int64_t T, int64_t H, void *h, void *n, float *stats, terrace_stream_t stream) {
+    return run_block_norm(y, y_dtype, residual, r_dtype, w_post, post_dtype, gate, gate_dtype, gate_kind, w_pre, pre_dtype,
+                          scale, eps, T, H, h, n, stats, (hipStream_t)stream);
+}
+
+size_t terrace_block_norm_grad_workspace(int64_t T, int64_t H) { return block_norm_grad_workspace(T, H); }
+
+int terrace_block_norm_grad(const void *y, int y_dtype, const void *residual, int r_dtype, const void *w_post,
+                            int post_dtype, const void *gate, int gate_dtype, int gate_kind, const void *w_pre,
+                            int pre_dtype, float scale, float eps, int64_t T, int64_t H, const float *stats,
+                            const void *dh, const void *dn, void *dy, void *d_residual, void *d_post, void *d_gate,
+                            void *d_pre, void *workspace, size_t workspace_bytes, terrace_stream_t stream) {
+    return run_block_norm_grad(y, y_dtype, residual, r_dtype, w_post, post_dtype, gate, gate_dtype, gate_kind, w_pre,
+                               pre_dtype, scale, eps, T, H, stats, dh, dn, dy, d_residual, d_post, d_gate, d_pre,
+                               workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -63,6 +63,25 @@ __device__ __forceinline__ int wave_inclusive_scan(int v) {
     return v;
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <typename V>
+__device__ __forceinline__ V ld_stream(const V *p) { return __builtin_nontemporal_load(p); }
+template <typename V>
+__device__ __forceinline__ void st_stream(V *p, V v) { __builtin_nontemporal_store(v, p); }
+
+template <typename V>
+__device__ __forceinline__ V zero_of() { return V(0); }
+template <>
+__device__ __forceinline__ u32x4 zero_of<u32x4>() { return u32x4{0u, 0u, 0u, 0u}; }
+
+// Row ids a caller hands in are never trusted with an address: an id is used only if it lies in [0, bound),
+// which one unsigned compare decides ((uint64_t)id < (uint64_t)bound is false for negative ids too).  An id
+// outside is a dead entry -- a zero row for a gather, no contribution for the combine, a copy not made for a
+// scatter.  The stage operators bound the planes their own index kernels wrote all the same.
+__device__ __forceinline__ bool row_in(int64_t id, int64_t bound) { return (uint64_t)id < (uint64_t)bound; }
+
 __device__ __forceinline__ float bf16_bits_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
 
 __device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) {
@@ -78,6 +97,72 @@ __device__ __forceinline__ float e4m3_to_f32(uint32_t c) {
     float mag = e ? __uint_as_float(((e + 120u) << 23) | (m << 20)) : (float)m * 0x1p-9f;
     if (e == 0xFu && m == 0x7u) mag = __uint_as_float(0x7FC00000u);
     return __uint_as_float(__float_as_uint(mag) | sign);
+}
+
+// N consecutive elements of a float row as fp32, and back with one rounding (to nearest even) each.  N = 8: `row` and
+// `at` on 16-byte boundaries, moved as 16-byte vectors; N = 1: any alignment the element type has.
+template <int DT, int N>
+__device__ __forceinline__ void load_floats(const void *row, int64_t at, float *f) {
+    static_assert(N == 1 || N == 8, "one element or one vector of eight");
+    if constexpr (DT == TERRACE_F32) {
+        if constexpr (N == 1) {
+            f[0] = ((const float *)row)[at];
+        } else {
+            const u32x4 *p = (const u32x4 *)((const float *)row + at);
+            const u32x4 a = ld_stream(p), b = ld_stream(p + 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[i] = __uint_as_float(a[i]);
+                f[4 + i] = __uint_as_float(b[i]);
+            }
+        }
+    } else {
+        uint32_t bits[N == 1 ? 1 : 4];
+        if constexpr (N == 1) {
+            bits[0] = ((const uint16_t *)row)[at];
+        } else {
+            const u32x4 a = ld_stream((const u32x4 *)((const uint16_t *)row + at));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bits[i] = a[i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t b = i & 1 ? bits[i / 2] >> 16 : bits[i / 2] & 0xFFFFu;
+            if constexpr (DT == TERRACE_BF16) f[i] = bf16_bits_to_f32(b);
+            else f[i] = __half2float(__ushort_as_half((unsigned short)b));
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ uint32_t to_bits16(float f) {
+    if constexpr (DT == TERRACE_BF16) return f32_to_bf16_bits(f) & 0xFFFFu;
+    else return __half_as_ushort(__float2half_rn(f));
+}
+template <int DT, int N>
+__device__ __forceinline__ void store_floats(void *row, int64_t at, const float *f) {
+    static_assert(N == 1 || N == 8, "one element or one vector of eight");
+    if constexpr (DT == TERRACE_F32) {
+        if constexpr (N == 1) {
+            ((float *)row)[at] = f[0];
+        } else {
+            u32x4 *p = (u32x4 *)((float *)row + at);
+            u32x4 a, b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] = __float_as_uint(f[i]);
+                b[i] = __float_as_uint(f[4 + i]);
+            }
+            st_stream(p, a);
+            st_stream(p + 1, b);
+        }
+    } else if constexpr (N == 1) {
+        ((uint16_t *)row)[at] = (uint16_t)to_bits16<DT>(f[0]);
+    } else {
+        u32x4 a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = to_bits16<DT>(f[2 * i]) | (to_bits16<DT>(f[2 * i + 1]) << 16);
+        st_stream((u32x4 *)((uint16_t *)row + at), a);
+    }
 }
 
 // A row-width argument of the C ABI may carry a pitch (TERRACE_ROW_PITCHED): `width` bytes of data every `pitch`

@@ -1,0 +1,500 @@
+// What stands between two blocks, in one pass over the rows: the RMS norm after a block, its gate and scale, the sum
+// with the residual, and the RMS norm before the next block.
+//
+//   p = y * inv1 * w_post            inv1 = 1 / sqrt(mean(y^2) + eps)      (without w_post: p = y)
+//   h = residual + scale * g * p     g: one per channel, one per token, or 1
+//   n = h * inv2 * w_pre             inv2 = 1 / sqrt(mean(h^2) + eps)      (without w_pre: no n)
+//
+// and the gradient.  With u = y * inv1, v = h * inv2, t = dn * w_pre and q = scale * g * p:
+//   dH = dh + inv2 * (t - v * mean(t v));  d_residual = dH;  dp = scale * g * dH
+//   d_y = inv1 * (dp * w_post - u * mean(dp w_post u));  d_w_post = sum dp u;  d_w_pre = sum dn v;  d_g = sum scale p dH
+// The two means need three sums that do not wait for each other -- sum(t v), sum((dh + inv2 t) q), sum(v q) -- because
+// sum(dH q) = sum((dh + inv2 t) q) - inv2 * mean(t v) * sum(v q), so a row costs one reduction.
+//
+// All arithmetic is fp32; every output is rounded once.  n comes from the unrounded h, and the gradient recomputes h
+// from y and the residual (which it reads instead of h: the same bytes), so no stored rounding enters it.
+#include "common.hpp"
+
+namespace terrace {
+
+constexpr int kNormThreads = 1024;
+
+struct NormArgs {
+    const void *y, *residual, *w_post, *gate, *w_pre;        // any but residual may be NULL
+    int post_dtype, gate_dtype, pre_dtype, gate_kind;
+    float scale, eps;
+    int64_t T, H;
+    int tpr;                                                 // threads per row: whole waves
+    int groups;                                              // rows a workgroup works on at a time
+};
+
+// A lane's share of a row: E elements as E / N pieces of N neighbours, piece i at (lane + i * tpr) * N.  The bits are kept as
+// loaded until they are used, which for 16-bit rows halves the registers of a row that is fetched ahead.
+template <int DT, int N, int E>
+struct Share {
+    static constexpr int kWords = N == 1 ? E : (DT == TERRACE_F32 ? E : E / 2);
+    uint32_t w[kWords];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const void *rows, int64_t row, int64_t H, int at, int tpr) {
+#pragma unroll
+        for (int i = 0; i < E / N; ++i) {
+            const int c = (at + i * tpr) * N;
+            const bool in = c < H;
+            if constexpr (N == 1) {
+                if constexpr (DT == TERRACE_F32) w[i] = in ? ((const uint32_t *)rows + row * H)[c] : 0u;
+                else w[i] = in ? (uint32_t)((const uint16_t *)rows + row * H)[c] : 0u;
+            } else {
+                constexpr int kVecs = DT == TERRACE_F32 ? 2 : 1, kBytes = DT == TERRACE_F32 ? 4 : 2;
+#pragma unroll
+                for (int v = 0; v < kVecs; ++v) {
+                    u32x4 x = zero_of<u32x4>();
+                    if (in) x = ld_stream((const u32x4 *)((const uint8_t *)rows + row * H * kBytes + c * kBytes) + v);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[(i * kVecs + v) * 4 + j] = x[j];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (DT == TERRACE_F32) {
+            return __uint_as_float(w[e]);
+        } else {
+            uint32_t b;
+            if constexpr (N == 1) b = w[e];
+            else b = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu;
+            if constexpr (DT == TERRACE_BF16) return bf16_bits_to_f32(b);
+            else return __half2float(__ushort_as_half((unsigned short)b));
+        }
+    }
+};
+
+template <int DT, int N, int E>
+__device__ __forceinline__ void store_share(void *rows, int64_t row, int64_t H, int at, int tpr, const float *f) {
+#pragma unroll
+    for (int i = 0; i < E / N; ++i) {
+        const int c = (at + i * tpr) * N;
+        if (c < H) store_floats<DT, N>((uint8_t *)rows + row * H * (DT == TERRACE_F32 ? 4 : 2), c, f + i * N);
+    }
+}
+
+// A vector over the channels (a weight, a gate) in the same shares; absent: `fill`.
+template <int N, int E>
+__device__ __forceinline__ void load_channels(const void *v, int dtype, int64_t H, int at, int tpr, float fill, float *f) {
+#pragma unroll
+    for (int i = 0; i < E / N; ++i) {
+        const int c = (at + i * tpr) * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[i * N + j] = fill;
+        if (v && c < H) {
+            if (dtype == TERRACE_F32) load_floats<TERRACE_F32, N>(v, c, f + i * N);
+            else if (dtype == TERRACE_BF16) load_floats<TERRACE_BF16, N>(v, c, f + i * N);
+            else load_floats<TERRACE_F16, N>(v, c, f + i * N);
+        }
+    }
+}
+
+__device__ __forceinline__ float load_scalar(const void *v, int dtype, int64_t i) {
+    float f;
+    if (dtype == TERRACE_F32) load_floats<TERRACE_F32, 1>(v, i, &f);
+    else if (dtype == TERRACE_BF16) load_floats<TERRACE_BF16, 1>(v, i, &f);
+    else load_floats<TERRACE_F16, 1>(v, i, &f);
+    return f;
+}
+
+// Sum of M values over the tpr threads of a row, in every thread; called by all threads of the workgroup.  `part` holds
+// M floats per wave; two buffers used in turn need no barrier between one sum and the next.
+template <int M>
+__device__ __forceinline__ void row_sum(float *v, float *part, int tpr) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) v[m] += __shfl_xor(v[m], d, kWave);
+    }
+    if (tpr == kWave) return;
+    const int w = wave_in_block(), n = tpr / kWave, w0 = w / n * n;
+    if (lane_id() == 0) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) part[w * M + m] = v[m];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < M; ++m) v[m] = 0.0f;
+    for (int i = 0; i < n; ++i) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] += part[(w0 + i) * M + m];
+    }
+}
+
+template <int TY, int TR, int N, int E>
+__global__ __launch_bounds__(kNormThreads) void block_norm_kernel(NormArgs a, void *__restrict__ h_out,
+                                                                  void *__restrict__ n_out, float *__restrict__ stats) {
+    __shared__ float part[2][kNormThreads / kWave];
+    const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / a.tpr);          // whole waves per row
+    const int at = (int)threadIdx.x - group * a.tpr;
+    const int64_t wanted = (int64_t)blockIdx.x * a.groups + group;
+    const bool mine = wanted < a.T;
+    const int64_t row = mine ? wanted : a.T - 1;             // an idle group reads a row that is there and writes none
+    const float inv_h = 1.0f / (float)a.H;
+    Share<TY, N, E> y;
+    Share<TR, N, E> r;
+    if (a.y) y.load(a.y, row, a.H, at, a.tpr);
+    else y.clear();
+    r.load(a.residual, row, a.H, at, a.tpr);
+    float h[E], inv1 = 1.0f, inv2 = 1.0f;
+    if (a.w_post) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s = __fmaf_rn(y.get(e), y.get(e), s);
+        row_sum<1>(&s, part[0], a.tpr);
+        inv1 = 1.0f / sqrtf(__fmaf_rn(s, inv_h, a.eps));
+    }
+    {
+        float w[E], g[E];
+        load_channels<N, E>(a.w_post, a.post_dtype, a.H, at, a.tpr, 1.0f, w);
+        float token = 1.0f;
+        if (a.gate_kind == TERRACE_GATE_TOKEN) token = load_scalar(a.gate, a.gate_dtype, row);
+        load_channels<N, E>(a.gate_kind == TERRACE_GATE_CHANNEL ? a.gate : nullptr, a.gate_dtype, a.H, at, a.tpr, token, g);
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[e] = a.y ? __fmaf_rn(a.scale * g[e], y.get(e) * inv1 * w[e], r.get(e)) : r.get(e);
+    }
+    if (mine && h_out) store_share<TR, N, E>(h_out, row, a.H, at, a.tpr, h);
+    if (a.w_pre) {
+        float s = 0.0f, w[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) s = __fmaf_rn(h[e], h[e], s);
+        load_channels<N, E>(a.w_pre, a.pre_dtype, a.H, at, a.tpr, 0.0f, w);
+        row_sum<1>(&s, part[1], a.tpr);
+        inv2 = 1.0f / sqrtf(__fmaf_rn(s, inv_h, a.eps));
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[e] = h[e] * inv2 * w[e];
+        if (mine) store_share<TY, N, E>(n_out, row, a.H, at, a.tpr, h);
+    }
+    if (mine && stats && at == 0) {
+        stats[2 * row] = inv1;
+        stats[2 * row + 1] = inv2;
+    }
+}
+
+// The gradient.  A workgroup walks the rows blockIdx.x * groups + group + i * gridDim.x * groups.  The next row is fetched
+// before the present one is reduced: the workgroup fills a CU, and without that nothing would be in flight while its
+// waves meet.  The vectors over the channels wait in LDS.  The sums over the rows stay in registers over the walk, two of
+// them, because d_w_post and the gradient of a gate per channel are both multiples of sum(dH u): each workgroup leaves one
+// row partial[2][gridDim.x][H] of sum(factor dH u) and sum(dn v), and norm_reduce_kernel adds those up in order.
+// WIDE (16 elements a lane): the sums are kept in the partial row itself, which the lane that owns the channel reads and
+// writes row by row, the vectors come from cache, and no row is fetched ahead.
+struct NormGrad {
+    const void *dh, *dn;                                     // either may be NULL
+    const float *stats;
+    void *dy, *d_residual, *d_token;                         // any may be NULL; d_token: the per-token gate's gradient
+    float *partial;
+    int want_z, want_v;
+};
+
+template <int N, int E, bool WIDE>
+__device__ __forceinline__ void take_channels(const void *v, int dtype, const float *lds, int64_t H, int at, int tpr,
+                                              float fill, float *f) {
+    if constexpr (WIDE) {
+        load_channels<N, E>(v, dtype, H, at, tpr, fill, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E / N; ++i) {
+            const int c = (at + i * tpr) * N;
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[i * N + j] = fill;
+            if (v && c < H) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) f[i * N + j] = lds[c + j];
+            }
+        }
+    }
+}
+
+template <int TY, int TR, int N, int E, bool WIDE>
+__global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs a, NormGrad d) {
+    __shared__ float part[2][kNormThreads / kWave * 3];
+    extern __shared__ float vectors[];                       // [3][H]: w_post, gate per channel, w_pre
+    const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / a.tpr);          // whole waves per row
+    const int at = (int)threadIdx.x - group * a.tpr;
+    const float inv_h = 1.0f / (float)a.H;
+    const int64_t stride = (int64_t)gridDim.x * a.groups;
+    const void *channel_gate = a.gate_kind == TERRACE_GATE_CHANNEL ? a.gate : nullptr;
+    float *lds_post = vectors, *lds_gate = vectors + a.H, *lds_pre = vectors + 2 * a.H;
+    if constexpr (!WIDE) {
+        for (int64_t c = threadIdx.x; c < a.H; c += blockDim.x) {
+            if (a.w_post) lds_post[c] = load_scalar(a.w_post, a.post_dtype, c);
+            if (channel_gate) lds_gate[c] = load_scalar(channel_gate, a.gate_dtype, c);
+            if (a.w_pre) lds_pre[c] = load_scalar(a.w_pre, a.pre_dtype, c);
+        }
+        __syncthreads();
+    }
+    float sum[2][WIDE ? 1 : E];
+    if constexpr (!WIDE) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[0][e] = sum[1][e] = 0.0f;
+    }
+    struct Row {
+        Share<TY, N, E> y, dn;
+        Share<TR, N, E> r, dh;
+        float inv1, inv2, token;
+    };
+    auto fetch = [&](int64_t row, Row &x) {
+        x.y.clear(), x.r.clear(), x.dh.clear(), x.dn.clear();
+        x.inv1 = x.inv2 = x.token = 1.0f;
+        if (row >= a.T) return;
+        if (a.y) x.y.load(a.y, row, a.H, at, a.tpr);
+        x.r.load(a.residual, row, a.H, at, a.tpr);
+        if (d.dh) x.dh.load(d.dh, row, a.H, at, a.tpr);
+        if (d.dn) x.dn.load(d.dn, row, a.H, at, a.tpr);
+        x.inv1 = d.stats[2 * row];
+        x.inv2 = d.stats[2 * row + 1];
+        if (a.gate_kind == TERRACE_GATE_TOKEN) x.token = load_scalar(a.gate, a.gate_dtype, row);
+    };
+    const int64_t first = (int64_t)blockIdx.x * a.groups;
+    Row cur, next;
+    fetch(first + group, cur);
+    int turn = 0;
+    for (int64_t base = first; base < a.T; base += stride) {
+        const int64_t row = base + group;
+        const bool mine = row < a.T;
+        if constexpr (!WIDE) fetch(row + stride, next);
+        float s[3] = {0.0f, 0.0f, 0.0f};
+        const float factor = a.scale * cur.token;            // scale, and the token's gate where there is one
+        float wp[E], gc[E], wn[E];
+        take_channels<N, E, WIDE>(a.w_post, a.post_dtype, lds_post, a.H, at, a.tpr, 1.0f, wp);
+        take_channels<N, E, WIDE>(channel_gate, a.gate_dtype, lds_gate, a.H, at, a.tpr, 1.0f, gc);
+        take_channels<N, E, WIDE>(a.w_pre, a.pre_dtype, lds_pre, a.H, at, a.tpr, 0.0f, wn);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float u = cur.y.get(e) * cur.inv1, q = gc[e] * (u * wp[e]);
+            const float h = __fmaf_rn(factor, q, cur.r.get(e)), v = h * cur.inv2, t = cur.dn.get(e) * wn[e];
+            s[0] = __fmaf_rn(t, v, s[0]);
+            s[1] = __fmaf_rn(__fmaf_rn(cur.inv2, t, cur.dh.get(e)), q, s[1]);
+            s[2] = __fmaf_rn(v, q, s[2]);
+        }
+        row_sum<3>(s, part[turn], a.tpr);
+        turn ^= 1;
+        const float mean_tv = s[0] * inv_h;
+        const float dot = __fmaf_rn(-cur.inv2 * mean_tv, s[2], s[1]);         // sum of dH * gate per channel * p
+        const float mean_u = factor * dot * inv_h;
+        take_channels<N, E, WIDE>(a.w_post, a.post_dtype, lds_post, a.H, at, a.tpr, 1.0f, wp);
+        take_channels<N, E, WIDE>(channel_gate, a.gate_dtype, lds_gate, a.H, at, a.tpr, 1.0f, gc);
+        take_channels<N, E, WIDE>(a.w_pre, a.pre_dtype, lds_pre, a.H, at, a.tpr, 0.0f, wn);
+        float o1[E], o2[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float u = cur.y.get(e) * cur.inv1;
+            const float h = __fmaf_rn(factor, gc[e] * (u * wp[e]), cur.r.get(e)), v = h * cur.inv2;
+            const float dn = cur.dn.get(e);
+            const float dH = __fmaf_rn(cur.inv2, __fmaf_rn(-v, mean_tv, dn * wn[e]), cur.dh.get(e));
+            const float z = factor * dH;
+            o1[e] = dH;
+            o2[e] = gc[e] * z;
+            if (a.w_post) o2[e] = cur.inv1 * __fmaf_rn(-u, mean_u, o2[e] * wp[e]);
+            if constexpr (!WIDE) {
+                sum[0][e] = __fmaf_rn(z, u, sum[0][e]);
+                sum[1][e] = __fmaf_rn(dn, v, sum[1][e]);
+            } else if (mine) {                               // one group: this lane alone touches the channel's cells
+                const int64_t c = ((int64_t)at + (int64_t)(e / N) * a.tpr) * N + e % N;
+                if (c < a.H) {
+                    float *cell = d.partial + (int64_t)blockIdx.x * a.H + c;
+                    if (d.want_z) *cell = base == first ? z * u : __fmaf_rn(z, u, *cell);
+                    cell += (int64_t)gridDim.x * a.H;
+                    if (d.want_v) *cell = base == first ? dn * v : __fmaf_rn(dn, v, *cell);
+                }
+            }
+        }
+        if (mine) {
+            if (d.d_residual) store_share<TR, N, E>(d.d_residual, row, a.H, at, a.tpr, o1);
+            if (d.dy) store_share<TY, N, E>(d.dy, row, a.H, at, a.tpr, o2);
+            if (d.d_token && at == 0) {
+                const float dg = a.scale * dot;
+                if (a.gate_dtype == TERRACE_F32) store_floats<TERRACE_F32, 1>(d.d_token, row, &dg);
+                else if (a.gate_dtype == TERRACE_BF16) store_floats<TERRACE_BF16, 1>(d.d_token, row, &dg);
+                else store_floats<TERRACE_F16, 1>(d.d_token, row, &dg);
+            }
+        }
+        if constexpr (WIDE) fetch(row + stride, cur);
+        else cur = next;
+    }
+    if constexpr (!WIDE) {
+        const int want[2] = {d.want_z, d.want_v};
+        __syncthreads();                                     // the vectors' LDS holds the joined sums from here on
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (!want[k]) continue;
+            float *out = d.partial + ((int64_t)k * gridDim.x + blockIdx.x) * a.H;
+            if (a.groups == 1) {
+                store_share<TERRACE_F32, N, E>(out, 0, a.H, at, a.tpr, sum[k]);
+                continue;
+            }
+            for (int g = 0; g < a.groups; ++g) {             // the row groups one after the other: a fixed order
+                if (group == g) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const int c = (at + (e / N) * a.tpr) * N + e % N;
+                        if (c < a.H) vectors[c] = g ? vectors[c] + sum[k][e] : sum[k][e];
+                    }
+                }
+                __syncthreads();
+            }
+            for (int64_t c = threadIdx.x; c < a.H; c += blockDim.x) out[c] = vectors[c];
+            __syncthreads();
+        }
+    }
+}
+
+// The workgroups' partial rows added up, 64 columns a workgroup: its 16 waves take every 16th partial row and are joined
+// in order.  blockIdx.y = 0: sum(factor dH u), which times the gate is d_w_post and times w_post is the gradient of a
+// gate per channel; 1: d_w_pre.
+struct NormReduce {
+    void *d_post, *d_gate, *d_pre;
+};
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(const float *__restrict__ partial, int rows, NormArgs a,
+                                                           NormReduce r) {
+    __shared__ float part[16][kWave];
+    const int k = blockIdx.y, w = wave_in_block(), lane = lane_id();
+    if (k == 0 ? !r.d_post && !r.d_gate : !r.d_pre) return;
+    const int64_t c = (int64_t)blockIdx.x * kWave + lane;
+    const float *p = partial + (int64_t)k * rows * a.H;
+    float v = 0.0f;
+    if (c < a.H) {
+#pragma unroll 8
+        for (int g = w; g < rows; g += 16) v += p[(int64_t)g * a.H + c];
+    }
+    part[w][lane] = v;
+    __syncthreads();
+    if (w || c >= a.H) return;
+    v = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v += part[x][lane];
+    auto put = [&](void *out, int dtype, float f) {
+        if (dtype == TERRACE_F32) store_floats<TERRACE_F32, 1>(out, c, &f);
+        else if (dtype == TERRACE_BF16) store_floats<TERRACE_BF16, 1>(out, c, &f);
+        else store_floats<TERRACE_F16, 1>(out, c, &f);
+    };
+    if (k == 1) {
+        put(r.d_pre, a.pre_dtype, v);
+        return;
+    }
+    if (r.d_post) put(r.d_post, a.post_dtype, a.gate_kind == TERRACE_GATE_CHANNEL ? v * load_scalar(a.gate, a.gate_dtype, c) : v);
+    if (r.d_gate) put(r.d_gate, a.gate_dtype, a.w_post ? v * load_scalar(a.w_post, a.post_dtype, c) : v);
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+constexpr int64_t kNormMaxH = 2 * 8 * kNormThreads;          // 16 elements a lane, rows in vectors of 8
+constexpr int64_t kNormMaxOdd = 8 * kNormThreads;            // 8 elements a lane
+constexpr int kNormGradBlocks = 256;                         // one workgroup a CU
+
+static bool norm_float(int d) { return d == TERRACE_F32 || d == TERRACE_BF16 || d == TERRACE_F16; }
+
+// 0 when the rows cannot be taken; else N * 100 + E
+static int norm_form(const NormArgs &a, uintptr_t bits) {
+    if (a.H % 8 == 0 && (bits & 15) == 0) return a.H <= kNormMaxOdd ? 808 : a.H <= kNormMaxH ? 816 : 0;
+    return a.H <= kNormMaxOdd ? 108 : 0;
+}
+
+static int norm_check(const NormArgs &a, int y_dtype, int r_dtype) {
+    if (a.T < 0 || a.H <= 0 || !norm_float(y_dtype) || !norm_float(r_dtype) ||
+        (r_dtype != y_dtype && r_dtype != TERRACE_F32) || a.gate_kind < TERRACE_GATE_NONE || a.gate_kind > TERRACE_GATE_TOKEN ||
+        (a.T > 0 && (a.gate_kind != TERRACE_GATE_NONE) != (a.gate != nullptr)) || (a.w_post && !norm_float(a.post_dtype)) ||
+        (a.gate && !norm_float(a.gate_dtype)) || (a.w_pre && !norm_float(a.pre_dtype)) || a.T >= ((int64_t)1 << 22) ||
+        (a.T > 0 && !a.y && (a.w_post || a.gate)))
+        return TERRACE_EINVAL;
+    return TERRACE_OK;
+}
+
+static void norm_shape(NormArgs &a, int form) {
+    const int per = form % 100;
+    a.tpr = (int)(((a.H + per - 1) / per + kWave - 1) / kWave * kWave);
+    a.groups = 1;
+}
+
+#define TERRACE_NORM_TYPES(CALL)                                                                  \
+    if (y_dtype == TERRACE_F32) { CALL(TERRACE_F32, TERRACE_F32); }                               \
+    else if (y_dtype == TERRACE_BF16 && r_dtype == TERRACE_BF16) { CALL(TERRACE_BF16, TERRACE_BF16); } \
+    else if (y_dtype == TERRACE_BF16) { CALL(TERRACE_BF16, TERRACE_F32); }                        \
+    else if (r_dtype == TERRACE_F16) { CALL(TERRACE_F16, TERRACE_F16); }                          \
+    else { CALL(TERRACE_F16, TERRACE_F32); }
+
+int run_block_norm(const void *y, int y_dtype, const void *residual, int r_dtype, const void *w_post, int post_dtype,
+                   const void *gate, int gate_dtype, int gate_kind, const void *w_pre, int pre_dtype, float scale,
+                   float eps, int64_t T, int64_t H, void *h, void *n, float *stats, hipStream_t s) {
+    NormArgs a{y, residual, w_post, gate, w_pre, post_dtype, gate_dtype, pre_dtype, gate_kind, scale, eps, T, H, 0, 1};
+    int rc = norm_check(a, y_dtype, r_dtype);
+    if (rc != TERRACE_OK) return rc;
+    uintptr_t bits = (uintptr_t)y | (uintptr_t)residual | (uintptr_t)w_post | (uintptr_t)w_pre | (uintptr_t)h | (uintptr_t)n;
+    if (gate_kind == TERRACE_GATE_CHANNEL) bits |= (uintptr_t)gate;
+    const int form = norm_form(a, bits);
+    if (!form) return TERRACE_EINVAL;
+    if (T == 0) return TERRACE_OK;
+    if (!residual || (y && !h) || (w_pre && !n)) return TERRACE_EINVAL;
+    norm_shape(a, form);
+    if (a.tpr < kBlock) a.groups = kBlock / a.tpr;
+    const unsigned grid = (unsigned)((T + a.groups - 1) / a.groups), threads = (unsigned)(a.tpr * a.groups);
+#define TERRACE_NORM(Y, R)                                                                          \
+    if (form == 808) block_norm_kernel<Y, R, 8, 8><<<grid, threads, 0, s>>>(a, h, n, stats);        \
+    else if (form == 816) block_norm_kernel<Y, R, 8, 16><<<grid, threads, 0, s>>>(a, h, n, stats);  \
+    else block_norm_kernel<Y, R, 1, 8><<<grid, threads, 0, s>>>(a, h, n, stats)
+    TERRACE_NORM_TYPES(TERRACE_NORM)
+#undef TERRACE_NORM
+    return check_launch();
+}
+
+static unsigned norm_grad_grid(int64_t T, int groups) {
+    const int64_t need = (T + groups - 1) / groups;
+    return (unsigned)(need < kNormGradBlocks ? need : kNormGradBlocks);
+}
+
+size_t block_norm_grad_workspace(int64_t T, int64_t H) {
+    if (T <= 0 || H <= 0 || H > kNormMaxH) return 256;
+    const int64_t grid = T < kNormGradBlocks ? T : kNormGradBlocks;
+    return align_up((size_t)(2 * grid * H) * sizeof(float), 256);
+}
+
+int run_block_norm_grad(const void *y, int y_dtype, const void *residual, int r_dtype, const void *w_post,
+                        int post_dtype, const void *gate, int gate_dtype, int gate_kind, const void *w_pre,
+                        int pre_dtype, float scale, float eps, int64_t T, int64_t H, const float *stats, const void *dh,
+                        const void *dn, void *dy, void *d_residual, void *d_post, void *d_gate, void *d_pre, void *ws,
+                        size_t ws_bytes, hipStream_t s) {
+    NormArgs a{y, residual, w_post, gate, w_pre, post_dtype, gate_dtype, pre_dtype, gate_kind, scale, eps, T, H, 0, 1};
+    int rc = norm_check(a, y_dtype, r_dtype);
+    if (rc != TERRACE_OK) return rc;
+    if ((d_post && !w_post) || (T > 0 && d_gate && !gate) || (d_pre && !w_pre) || (T > 0 && dy && !y) || (dn && !w_pre))
+        return TERRACE_EINVAL;
+    uintptr_t bits = (uintptr_t)y | (uintptr_t)residual | (uintptr_t)w_post | (uintptr_t)w_pre | (uintptr_t)dh |
+                     (uintptr_t)dn | (uintptr_t)dy | (uintptr_t)d_residual | (uintptr_t)ws;
+    if (gate_kind == TERRACE_GATE_CHANNEL) bits |= (uintptr_t)gate;
+    const int form = norm_form(a, bits);
+    if (!form || ((uintptr_t)ws & 3)) return TERRACE_EINVAL;
+    const bool channel_gate = gate_kind == TERRACE_GATE_CHANNEL;
+    const NormReduce red{d_post, channel_gate ? d_gate : nullptr, d_pre};
+    const bool want_z = red.d_post || red.d_gate, want_v = red.d_pre != nullptr, sums = want_z || want_v;
+    if (sums && (!ws || ws_bytes < block_norm_grad_workspace(T, H))) return ws ? TERRACE_ENOSPC : TERRACE_EINVAL;
+    unsigned grid = 0;
+    if (T > 0) {
+        if (!residual || !stats) return TERRACE_EINVAL;
+        norm_shape(a, form);
+        if (form != 816) a.groups = kNormThreads / a.tpr;
+        grid = norm_grad_grid(T, a.groups);
+        const NormGrad d{dh, dn, stats, dy, d_residual, gate_kind == TERRACE_GATE_TOKEN ? d_gate : nullptr, (float *)ws, want_z,
+                         want_v};
+        const unsigned threads = (unsigned)(a.tpr * a.groups);
+        const size_t lds = form == 816 ? 0 : (size_t)(3 * H) * sizeof(float);
+#define TERRACE_NORM(Y, R)                                                                            \
+    if (form == 808) block_norm_grad_kernel<Y, R, 8, 8, false><<<grid, threads, lds, s>>>(a, d);      \
+    else if (form == 816) block_norm_grad_kernel<Y, R, 8, 16, true><<<grid, threads, lds, s>>>(a, d); \
+    else block_norm_grad_kernel<Y, R, 1, 8, false><<<grid, threads, lds, s>>>(a, d)
+        TERRACE_NORM_TYPES(TERRACE_NORM)
+#undef TERRACE_NORM
+    }
+    if (sums)
+        norm_reduce_kernel<<<dim3((unsigned)((H + kWave - 1) / kWave), 2), 1024, 0, s>>>((const float *)ws, (int)grid, a, red);
+    return check_launch();
+}
+
+}  // namespace terrace

@@ -15,19 +15,6 @@
 
 namespace terrace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
-template <typename V>
-__device__ __forceinline__ V ld_stream(const V *p) { return __builtin_nontemporal_load(p); }
-template <typename V>
-__device__ __forceinline__ void st_stream(V *p, V v) { __builtin_nontemporal_store(v, p); }
-
-template <typename V>
-__device__ __forceinline__ V zero_of() { return V(0); }
-template <>
-__device__ __forceinline__ u32x4 zero_of<u32x4>() { return u32x4{0u, 0u, 0u, 0u}; }
-
 // ---------------------------------------------------------------------------------------------
 // streaming copy
 // ---------------------------------------------------------------------------------------------
@@ -159,12 +146,6 @@ int launch_stream_probe(int kind, const void *x, void *y, size_t nbytes, hipStre
     }
     return check_launch();
 }
-
-// Row ids a caller hands in are never trusted with an address: an id is used only if it lies in [0, bound),
-// which one unsigned compare decides ((uint64_t)id < (uint64_t)bound is false for negative ids too).  An id
-// outside is a dead entry -- a zero row for a gather, no contribution for the combine, a copy not made for a
-// scatter.  The stage operators bound the planes their own index kernels wrote all the same.
-__device__ __forceinline__ bool row_in(int64_t id, int64_t bound) { return (uint64_t)id < (uint64_t)bound; }
 
 // ---------------------------------------------------------------------------------------------
 // scatter: one read, fan writes

@@ -108,6 +108,16 @@ struct KeyAffine {           // bucket = (plane[item] - sub) / div
     }
 };
 
+struct KeyExpert {           // bucket = expert id; a negative id is a pair without an expert, one past the end is reported
+    const int64_t *plane;
+    int n_experts;
+    __device__ __forceinline__ int64_t fetch(int64_t item) const { return plane[item]; }
+    __device__ __forceinline__ int bucket(int64_t, int64_t v, bool *bad) const {
+        if (v >= n_experts) *bad = true;
+        return v < 0 || v >= n_experts ? -1 : (int)v;
+    }
+};
+
 // A token's k expert ids and their nodes, in registers when k <= KMAX (KMAX > 0), else re-read
 // through L1.  Padding entries hold INT_MAX so they rank after every real id.  An id is narrowed only after its
 // 64-bit value has been bounded: a negative one becomes -1 and one beyond the int range INT_MAX - 1, so neither
@@ -496,6 +506,12 @@ void launch_scan(const Units &u, int32_t *table, const TableOut &out, int32_t *s
 // ---------------------------------------------------------------------------------------------
 // rank
 // ---------------------------------------------------------------------------------------------
+// An emitter with a skipped(item) member hears of the items its key functor gave no bucket (a negative key).
+template <typename EmitFn, typename = void>
+struct takes_skipped : std::false_type {};
+template <typename EmitFn>
+struct takes_skipped<EmitFn, std::void_t<decltype(&EmitFn::skipped)>> : std::true_type {};
+
 template <typename KeyFn, typename EmitFn, int CH>
 __global__ __launch_bounds__(kSortBlockMax) void rank_kernel(KeyFn key_of, EmitFn emit, Units u,
                                                              int32_t *__restrict__ table, TableOut out,
@@ -636,6 +652,9 @@ __global__ __launch_bounds__(kSortBlockMax) void rank_kernel(KeyFn key_of, EmitF
     for (int c = 0; c < CH; ++c) {
         const int64_t item = first + (int64_t)c * kWave + lane;
         if (keys[c] >= 0) fault |= emit(item, keys[c], dests[c], fetched[c], pre[c], start, tally);
+        if constexpr (takes_skipped<EmitFn>::value) {
+            if (keys[c] < 0 && item < u.n_items) emit.skipped(item);
+        }
     }
     if constexpr (EmitFn::kFills) emit.fill(unit, u.n_units, lane, start);
     if (!status) return;
@@ -770,6 +789,24 @@ struct EmitHopB {            // arrival + expert-order regroup in one placement 
             }
         }
         return 0;
+    }
+};
+
+struct EmitExpert {          // where[p] = place of pair p in expert order, -1 for a pair without an expert
+    int64_t *where;
+    int32_t *pos32;
+    static constexpr bool kTallies = false;
+    static constexpr bool kFills = false;
+    typedef NoPre Pre;
+    __device__ __forceinline__ Pre fetch(int64_t) const { return Pre{}; }
+    __device__ __forceinline__ int operator()(int64_t p, int, int32_t dest, int64_t, Pre, const int32_t *, int *) const {
+        where[p] = dest;
+        pos32[p] = dest;
+        return 0;
+    }
+    __device__ __forceinline__ void skipped(int64_t p) const {
+        where[p] = -1;
+        pos32[p] = -1;
     }
 };
 
@@ -1401,6 +1438,31 @@ int run_hopb_scatter_move(const void *rx, int64_t R, int64_t row_bytes, int quot
         if (rc != TERRACE_OK) return rc;
     }
     return launch_scatter_rows<int32_t>(rx, permuted, pos32, R, quota, row_bytes, places, s);
+}
+
+// ---- (token, expert) pairs straight to expert order ---------------------------------------------
+size_t expert_index_workspace(int64_t P, int n_experts) {
+    if (P <= 0 || n_experts <= 0 || n_experts > kMaxBuckets) return 256;
+    return units_table_bytes(make_units(P, n_experts)) + align_up((size_t)P * sizeof(int32_t), 256);
+}
+
+// The stable sort of P >= 1 pairs by expert: where [P], tokens_per_expert [n_experts] and offsets [n_experts + 1] as
+// terrace_expert_sort documents them (offsets[n_experts] is left to the caller: `*live` points at that total);
+// `*pos32` is the int32 twin of `where` for the row mover.  The caller has checked sizes and the workspace.
+int run_expert_index(const int64_t *expert_idx, int64_t P, int n_experts, int64_t *where, int64_t *tokens_per_expert,
+                     int64_t *offsets, int32_t *status, void *ws, const int32_t **pos32, const int32_t **live,
+                     hipStream_t s) {
+    const Units u = make_units(P, n_experts);
+    int32_t *table = (int32_t *)ws;
+    int32_t *pos = (int32_t *)((char *)ws + units_table_bytes(u));
+    KeyExpert key{expert_idx, n_experts};
+    EmitExpert emit{where, pos};
+    TableOut out;
+    out.hist_i64 = tokens_per_expert;
+    out.offsets_i64 = offsets;
+    *pos32 = pos;
+    *live = table + units_start_at(u) + n_experts;
+    return run_sort(key, emit, u, table, out, status, true, s);
 }
 
 // ---- expert-order regroup ---------------------------------------------------------------------

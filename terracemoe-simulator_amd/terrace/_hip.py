@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import glob
 import os
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -23,6 +23,7 @@ MODE_CODES = {"full": 0, "group_limited": 1, "quota_only": 2, "global_topk": 3}
 FORCE_GENERIC = 0x100
 GATES_FLAG = {torch.float32: 0, torch.bfloat16: 0x200, torch.float16: 0x400}
 PROBE_READ, PROBE_WRITE, PROBE_SUM8, PROBE_COPY = 0, 1, 2, 3
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN = 0, 1, 2
 FAULT_ID_RANGE, FAULT_QUOTA, FAULT_FANOUT = 1, 2, 4
 # enum terrace_dispatch_plane, in order
 DISPATCH_PLANES = ("mask", "gate_rows", "u_src", "node_counts", "u_node", "inverse", "node_offsets", "pair_table",
@@ -31,7 +32,7 @@ DISPATCH_PLANES = ("mask", "gate_rows", "u_src", "node_counts", "u_node", "inver
                    "kept_per_expert", "status_regroup")
 STATUS_WORDS = 4
 
-_P, _I, _L, _Z = c_void_p, c_int, c_int64, c_size_t
+_P, _I, _L, _Z, _F = c_void_p, c_int, c_int64, c_size_t, c_float
 
 # name -> (restype, argtypes); must list every function include/terrace_hip.h declares
 SIGNATURES = {
@@ -94,6 +95,16 @@ SIGNATURES = {
     "terrace_hopa_send_splits": (_I, [_P, _I, _I, _I, _P, _P]),
     "terrace_dispatch_workspace": (_Z, [_L, _I, _I, _I, _I, _I, _L, _I]),
     "terrace_dispatch": (_I, [_P, _P, _P, _L, _L, _I, _I, _I, _I, _I, _I, _L, _I, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "terrace_expert_sort_workspace": (_Z, [_L, _I, _I]),
+    "terrace_expert_sort": (_I, [_P, _P, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "terrace_expert_unsort_grad": (_I, [_P, _I, _P, _I, _P, _P, _I, _L, _I, _L, _L, _P, _P, _P, _P]),
+    "terrace_w4_packed_bytes": (_Z, [_I, _L, _L, _I, _I]),
+    "terrace_w4_pack": (_I, [_P, _P, _P, _I, _L, _L, _I, _P, _P, _P, _P]),
+    "terrace_w4_linear": (_I, [_P, _I, _L, _P, _P, _P, _P, _I, _L, _L, _I, _I, _P, _P]),
+    "terrace_block_norm": (_I, [_P, _I, _P, _I, _P, _I, _P, _I, _I, _P, _I, _F, _F, _L, _L, _P, _P, _P, _P]),
+    "terrace_block_norm_grad_workspace": (_Z, [_L, _L]),
+    "terrace_block_norm_grad": (_I, [_P, _I, _P, _I, _P, _I, _P, _I, _I, _P, _I, _F, _F, _L, _L,
+                                     _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "terrace_static_scratch_bytes": (_Z, []),
     "terrace_static_init": (_I, []),
     "terrace_k1_arrival_static": (_I, [_P, _P, _P, _L, _L, _I, _I, _I, _I, _I,

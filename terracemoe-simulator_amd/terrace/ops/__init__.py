@@ -1245,6 +1245,9 @@ def k1_arrival_ref(rx, rslot, rgate, quota: int, epr: int, rpn: int, my_local: i
     return k1_arrival(rx, rslot, rgate, quota, epr, rpn, my_local)
 
 
+from .experts import (ExpertPlan, W4Weights, block_norm, expert_linear_w4, expert_sort,        # noqa: E402
+                      expert_unsort, w4_pack)
+
 __all__ = [
     "OpsLoadError", "OpsState", "TerracePassthroughFn", "TerraceK1ArrivalFn", "TerraceK2PackFn",
     "custom_ops_enabled", "k1_arrival", "k1_arrival_ref", "k1_arrival_segment", "k2_pack", "passthrough", "reset",
@@ -1253,4 +1256,5 @@ __all__ = [
     "plan_general", "build_mask", "scatter_elems", "expand_mask", "arrival_pairs", "routing_map_topk", "segment_table", "pair_places",
     "wire_words", "k2_pack_wire", "k1_arrival_wire", "regroup_wire", "hopb_scatter", "hopb_scatter_move",
     "k1_arrival_static",
+    "ExpertPlan", "W4Weights", "block_norm", "expert_linear_w4", "expert_sort", "expert_unsort", "w4_pack",
 ]
