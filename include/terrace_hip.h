@@ -531,7 +531,7 @@ TERRACE_API int terrace_w4_pack(const void *codes, const void *scales, const voi
 /* out[i] = W[e] x[i] for the rows i of expert e: x [P,K] and out [P,N] of dtype (BF16 or F16, the scales' type too),
  * rows in expert order, tokens_per_expert [n_experts] i64 (NULL with one expert: all rows are its rows).  swiglu != 0: N is even and out [P,N/2] =
  * silu(first half of the columns) * second half, taken before the one rounding.  Sums are fp32.  Rows past the last
- * expert's are written as zeros.  Counts below 0 are taken as 0, and none reaches past row P.  x and the packed codes on 16 bytes.
+ * expert's are written as zeros.  Counts below 0 are taken as 0, and none reaches past row P.  x and the packed planes on 16 bytes.
  * Made for few rows per expert (every 16, 32 or 64 rows read the expert's weights once). */
 TERRACE_API int terrace_w4_linear(const void *x, int dtype, int64_t P, const int64_t *tokens_per_expert,
                                   const void *packed_codes, const void *packed_scales, const void *packed_zeros,
@@ -544,7 +544,7 @@ TERRACE_API int terrace_w4_linear(const void *x, int dtype, int64_t P, const int
  *   w_post [H] (NULL: p = y), gate [H] or [T] by gate_kind (NULL with TERRACE_GATE_NONE), w_pre [H] (NULL: no n).
  *   y NULL (with w_post and gate NULL): only the norm before a block, h = residual (h may then be NULL).
  *   stats [T,2] f32 (may be NULL): 1/rms of y and of h, for terrace_block_norm_grad.
- * H up to 16384 where it is a multiple of 8 and every row and weight lies on 16 bytes, up to 8192 otherwise. */
+ * H up to 16384; rows and vectors of whole 16 bytes on 16-byte boundaries take the aligned path. */
 enum terrace_gate_kind { TERRACE_GATE_NONE = 0, TERRACE_GATE_CHANNEL = 1, TERRACE_GATE_TOKEN = 2 };
 TERRACE_API int terrace_block_norm(const void *y, int y_dtype, const void *residual, int r_dtype, const void *w_post,
                                    int post_dtype, const void *gate, int gate_dtype, int gate_kind, const void *w_pre,

@@ -82,6 +82,25 @@ __device__ __forceinline__ u32x4 zero_of<u32x4>() { return u32x4{0u, 0u, 0u, 0u}
 // scatter.  The stage operators bound the planes their own index kernels wrote all the same.
 __device__ __forceinline__ bool row_in(int64_t id, int64_t bound) { return (uint64_t)id < (uint64_t)bound; }
 
+// Sum over the wave, in every lane: four rotations inside the rows of 16 lanes, then the rows' totals broadcast upwards
+// to the last lane -- register traffic only, where a butterfly of shuffles goes through LDS six times.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ float row16_sum(float v) {        // every lane: the sum of its row of 16
+    v = dpp_add<0x128, 0xF>(v);                              // row_ror:8
+    v = dpp_add<0x124, 0xF>(v);
+    v = dpp_add<0x122, 0xF>(v);
+    return dpp_add<0x121, 0xF>(v);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = row16_sum(v);
+    v = dpp_add<0x142, 0xA>(v);                              // row_bcast:15 into rows 1 and 3
+    v = dpp_add<0x143, 0xC>(v);                              // row_bcast:31 into rows 2 and 3
+    return __int_as_float(read_lane(__float_as_int(v), kWave - 1));
+}
+
 __device__ __forceinline__ float bf16_bits_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
 
 __device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) {
@@ -133,11 +152,19 @@ __device__ __forceinline__ void load_floats(const void *row, int64_t at, float *
         }
     }
 }
+// Two floats rounded (nearest even) to the halves of a register; bf16 pairs are one instruction on this part.
 template <int DT>
-__device__ __forceinline__ uint32_t to_bits16(float f) {
-    if constexpr (DT == TERRACE_BF16) return f32_to_bf16_bits(f) & 0xFFFFu;
-    else return __half_as_ushort(__float2half_rn(f));
+__device__ __forceinline__ uint32_t to_bits16x2(float lo, float hi) {
+    if constexpr (DT == TERRACE_BF16) {
+        typedef float f32x2_t __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo, hi}), bf16x2_t));
+    } else {
+        return (uint32_t)__half_as_ushort(__float2half_rn(lo)) | ((uint32_t)__half_as_ushort(__float2half_rn(hi)) << 16);
+    }
 }
+template <int DT>
+__device__ __forceinline__ uint32_t to_bits16(float f) { return to_bits16x2<DT>(f, 0.0f) & 0xFFFFu; }
 template <int DT, int N>
 __device__ __forceinline__ void store_floats(void *row, int64_t at, const float *f) {
     static_assert(N == 1 || N == 8, "one element or one vector of eight");
@@ -160,7 +187,7 @@ __device__ __forceinline__ void store_floats(void *row, int64_t at, const float 
     } else {
         u32x4 a;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = to_bits16<DT>(f[2 * i]) | (to_bits16<DT>(f[2 * i + 1]) << 16);
+        for (int i = 0; i < 4; ++i) a[i] = to_bits16x2<DT>(f[2 * i], f[2 * i + 1]);
         st_stream((u32x4 *)((uint16_t *)row + at), a);
     }
 }

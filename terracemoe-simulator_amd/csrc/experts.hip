@@ -275,9 +275,7 @@ __global__ __launch_bounds__(kBlock) void expert_unsort_grad_kernel(
         if (!d_weights) continue;
 #pragma unroll
         for (int j = 0; j < kGradFan; ++j) {
-            float v = sum[j];
-#pragma unroll
-            for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d, kWave);
+            const float v = wave_sum(sum[j]);
             if (lane_id() == 0) part[wave_in_block()][j] = v;
         }
         __syncthreads();

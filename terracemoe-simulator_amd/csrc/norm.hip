@@ -17,7 +17,7 @@
 
 namespace terrace {
 
-constexpr int kNormThreads = 1024;
+constexpr int kNormThreads = 1024, kNormWaves = kNormThreads / kWave;
 
 struct NormArgs {
     const void *y, *residual, *w_post, *gate, *w_pre;        // any but residual may be NULL
@@ -28,70 +28,118 @@ struct NormArgs {
     int groups;                                              // rows a workgroup works on at a time
 };
 
-// A lane's share of a row: E elements as E / N pieces of N neighbours, piece i at (lane + i * tpr) * N.  The bits are kept as
-// loaded until they are used, which for 16-bit rows halves the registers of a row that is fetched ahead.
-template <int DT, int N, int E>
+// A lane's share of a row: E elements as E / 8 pieces of 8 neighbours, piece i at (lane + i * tpr) * 8.  The bits are kept
+// as loaded until they are used, which for 16-bit rows halves the registers of a row that is fetched ahead.  ALIGNED:
+// rows are multiples of 8 elements on 16-byte boundaries; otherwise a piece is loaded and stored as a vector with the
+// alignment of its elements, and the last piece of a row element by element.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_word __attribute__((ext_vector_type(4), aligned(4)));
+
+template <int DT, bool ALIGNED>
+__device__ __forceinline__ void load_piece(const uint8_t *row, int c, int64_t H, uint32_t *w) {
+    constexpr int kVecs = DT == TERRACE_F32 ? 2 : 1, kBytes = DT == TERRACE_F32 ? 4 : 2;
+#pragma unroll
+    for (int j = 0; j < 4 * kVecs; ++j) w[j] = 0;
+    if (ALIGNED ? c < H : c + 8 <= H) {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const uint8_t *p = row + c * kBytes + v * 16;
+            u32x4 x;
+            if constexpr (ALIGNED) x = ld_stream((const u32x4 *)p);
+            else if constexpr (DT == TERRACE_F32) x = *(const u32x4_word *)p;
+            else x = *(const u32x4_any *)p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[4 * v + j] = x[j];
+        }
+    } else if (!ALIGNED && c < H) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (c + j >= H) continue;
+            if constexpr (DT == TERRACE_F32) w[j] = ((const uint32_t *)row)[c + j];
+            else w[j / 2] |= (uint32_t)((const uint16_t *)row)[c + j] << (j & 1 ? 16 : 0);
+        }
+    }
+}
+
+template <int DT, bool ALIGNED, int E>
 struct Share {
-    static constexpr int kWords = N == 1 ? E : (DT == TERRACE_F32 ? E : E / 2);
-    uint32_t w[kWords];
+    static constexpr int kPiece = DT == TERRACE_F32 ? 8 : 4;
+    uint32_t w[E / 8 * kPiece];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = 0;
+        for (int i = 0; i < E / 8 * kPiece; ++i) w[i] = 0;
     }
     __device__ __forceinline__ void load(const void *rows, int64_t row, int64_t H, int at, int tpr) {
 #pragma unroll
-        for (int i = 0; i < E / N; ++i) {
-            const int c = (at + i * tpr) * N;
-            const bool in = c < H;
-            if constexpr (N == 1) {
-                if constexpr (DT == TERRACE_F32) w[i] = in ? ((const uint32_t *)rows + row * H)[c] : 0u;
-                else w[i] = in ? (uint32_t)((const uint16_t *)rows + row * H)[c] : 0u;
-            } else {
-                constexpr int kVecs = DT == TERRACE_F32 ? 2 : 1, kBytes = DT == TERRACE_F32 ? 4 : 2;
-#pragma unroll
-                for (int v = 0; v < kVecs; ++v) {
-                    u32x4 x = zero_of<u32x4>();
-                    if (in) x = ld_stream((const u32x4 *)((const uint8_t *)rows + row * H * kBytes + c * kBytes) + v);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w[(i * kVecs + v) * 4 + j] = x[j];
-                }
-            }
-        }
+        for (int i = 0; i < E / 8; ++i)
+            load_piece<DT, ALIGNED>((const uint8_t *)rows + row * H * (DT == TERRACE_F32 ? 4 : 2), (at + i * tpr) * 8, H,
+                                    w + i * kPiece);
     }
     __device__ __forceinline__ float get(int e) const {
         if constexpr (DT == TERRACE_F32) {
             return __uint_as_float(w[e]);
         } else {
-            uint32_t b;
-            if constexpr (N == 1) b = w[e];
-            else b = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu;
+            const uint32_t b = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu;
             if constexpr (DT == TERRACE_BF16) return bf16_bits_to_f32(b);
             else return __half2float(__ushort_as_half((unsigned short)b));
         }
     }
 };
 
-template <int DT, int N, int E>
+template <int DT, bool ALIGNED, int E>
 __device__ __forceinline__ void store_share(void *rows, int64_t row, int64_t H, int at, int tpr, const float *f) {
+    uint8_t *base = (uint8_t *)rows + row * H * (DT == TERRACE_F32 ? 4 : 2);
 #pragma unroll
-    for (int i = 0; i < E / N; ++i) {
-        const int c = (at + i * tpr) * N;
-        if (c < H) store_floats<DT, N>((uint8_t *)rows + row * H * (DT == TERRACE_F32 ? 4 : 2), c, f + i * N);
+    for (int i = 0; i < E / 8; ++i) {
+        const int c = (at + i * tpr) * 8;
+        if constexpr (ALIGNED) {
+            if (c < H) store_floats<DT, 8>(base, c, f + i * 8);
+        } else if (c + 8 <= H) {
+            if constexpr (DT == TERRACE_F32) {
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    u32x4 x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = __float_as_uint(f[i * 8 + 4 * v + j]);
+                    *(u32x4_word *)(base + c * 4 + v * 16) = x;
+                }
+            } else {
+                u32x4 x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = to_bits16x2<DT>(f[i * 8 + 2 * j], f[i * 8 + 2 * j + 1]);
+                *(u32x4_any *)(base + c * 2) = x;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (c + j < H) store_floats<DT, 1>(base, c + j, f + i * 8 + j);
+            }
+        }
     }
 }
 
 // A vector over the channels (a weight, a gate) in the same shares; absent: `fill`.
-template <int N, int E>
+template <bool ALIGNED, int E>
 __device__ __forceinline__ void load_channels(const void *v, int dtype, int64_t H, int at, int tpr, float fill, float *f) {
 #pragma unroll
-    for (int i = 0; i < E / N; ++i) {
-        const int c = (at + i * tpr) * N;
+    for (int i = 0; i < E / 8; ++i) {
+        const int c = (at + i * tpr) * 8;
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[i * N + j] = fill;
-        if (v && c < H) {
-            if (dtype == TERRACE_F32) load_floats<TERRACE_F32, N>(v, c, f + i * N);
-            else if (dtype == TERRACE_BF16) load_floats<TERRACE_BF16, N>(v, c, f + i * N);
-            else load_floats<TERRACE_F16, N>(v, c, f + i * N);
+        for (int j = 0; j < 8; ++j) f[i * 8 + j] = fill;
+        if (!v) continue;
+        if constexpr (ALIGNED) {
+            if (c >= H) continue;
+            if (dtype == TERRACE_F32) load_floats<TERRACE_F32, 8>(v, c, f + i * 8);
+            else if (dtype == TERRACE_BF16) load_floats<TERRACE_BF16, 8>(v, c, f + i * 8);
+            else load_floats<TERRACE_F16, 8>(v, c, f + i * 8);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (c + j >= H) continue;
+                if (dtype == TERRACE_F32) load_floats<TERRACE_F32, 1>(v, c + j, f + i * 8 + j);
+                else if (dtype == TERRACE_BF16) load_floats<TERRACE_BF16, 1>(v, c + j, f + i * 8 + j);
+                else load_floats<TERRACE_F16, 1>(v, c + j, f + i * 8 + j);
+            }
         }
     }
 }
@@ -109,72 +157,85 @@ __device__ __forceinline__ float load_scalar(const void *v, int dtype, int64_t i
 template <int M>
 __device__ __forceinline__ void row_sum(float *v, float *part, int tpr) {
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) v[m] += __shfl_xor(v[m], d, kWave);
-    }
+    for (int m = 0; m < M; ++m) v[m] = wave_sum(v[m]);
     if (tpr == kWave) return;
-    const int w = wave_in_block(), n = tpr / kWave, w0 = w / n * n;
+    const int w = wave_in_block(), n = tpr / kWave, w0 = w / n * n, lane = lane_id() & 15;       // n <= 16 waves
     if (lane_id() == 0) {
 #pragma unroll
-        for (int m = 0; m < M; ++m) part[w * M + m] = v[m];
+        for (int m = 0; m < M; ++m) part[m * kNormWaves + w] = v[m];
     }
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < M; ++m) v[m] = 0.0f;
-    for (int i = 0; i < n; ++i) {
-#pragma unroll
-        for (int m = 0; m < M; ++m) v[m] += part[(w0 + i) * M + m];
-    }
+    for (int m = 0; m < M; ++m) v[m] = row16_sum(lane < n ? part[m * kNormWaves + w0 + lane] : 0.0f);
 }
 
-template <int TY, int TR, int N, int E>
+// A workgroup walks the rows (blockIdx.x + i * gridDim.x) * groups + group and fetches the next row before the present one
+// is reduced, so that something is in flight while its waves meet.
+template <int TY, int TR, bool ALIGNED, int E>
 __global__ __launch_bounds__(kNormThreads) void block_norm_kernel(NormArgs a, void *__restrict__ h_out,
                                                                   void *__restrict__ n_out, float *__restrict__ stats) {
-    __shared__ float part[2][kNormThreads / kWave];
+    __shared__ float part[2][kNormWaves];
     const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / a.tpr);          // whole waves per row
     const int at = (int)threadIdx.x - group * a.tpr;
-    const int64_t wanted = (int64_t)blockIdx.x * a.groups + group;
-    const bool mine = wanted < a.T;
-    const int64_t row = mine ? wanted : a.T - 1;             // an idle group reads a row that is there and writes none
     const float inv_h = 1.0f / (float)a.H;
-    Share<TY, N, E> y;
-    Share<TR, N, E> r;
-    if (a.y) y.load(a.y, row, a.H, at, a.tpr);
-    else y.clear();
-    r.load(a.residual, row, a.H, at, a.tpr);
-    float h[E], inv1 = 1.0f, inv2 = 1.0f;
-    if (a.w_post) {
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s = __fmaf_rn(y.get(e), y.get(e), s);
-        row_sum<1>(&s, part[0], a.tpr);
-        inv1 = 1.0f / sqrtf(__fmaf_rn(s, inv_h, a.eps));
-    }
+    const int64_t stride = (int64_t)gridDim.x * a.groups;
+    struct Row {
+        Share<TY, ALIGNED, E> y;
+        Share<TR, ALIGNED, E> r;
+        float token;
+    };
+    auto fetch = [&](int64_t row, Row &x) {
+        x.y.clear(), x.r.clear();
+        x.token = 1.0f;
+        if (row >= a.T) return;
+        if (a.y) x.y.load(a.y, row, a.H, at, a.tpr);
+        x.r.load(a.residual, row, a.H, at, a.tpr);
+        if (a.gate_kind == TERRACE_GATE_TOKEN) x.token = load_scalar(a.gate, a.gate_dtype, row);
+    };
+    const int64_t first = (int64_t)blockIdx.x * a.groups;
+    Row cur, next;
+    fetch(first + group, cur);
+    float w[E], wn[E];                                       // scale, norm weight and gate per channel; the norm before
+    load_channels<ALIGNED, E>(a.w_post, a.post_dtype, a.H, at, a.tpr, 1.0f, w);
     {
-        float w[E], g[E];
-        load_channels<N, E>(a.w_post, a.post_dtype, a.H, at, a.tpr, 1.0f, w);
-        float token = 1.0f;
-        if (a.gate_kind == TERRACE_GATE_TOKEN) token = load_scalar(a.gate, a.gate_dtype, row);
-        load_channels<N, E>(a.gate_kind == TERRACE_GATE_CHANNEL ? a.gate : nullptr, a.gate_dtype, a.H, at, a.tpr, token, g);
+        float g[E];
+        load_channels<ALIGNED, E>(a.gate_kind == TERRACE_GATE_CHANNEL ? a.gate : nullptr, a.gate_dtype, a.H, at, a.tpr, 1.0f, g);
 #pragma unroll
-        for (int e = 0; e < E; ++e) h[e] = a.y ? __fmaf_rn(a.scale * g[e], y.get(e) * inv1 * w[e], r.get(e)) : r.get(e);
+        for (int e = 0; e < E; ++e) w[e] *= a.scale * g[e];
     }
-    if (mine && h_out) store_share<TR, N, E>(h_out, row, a.H, at, a.tpr, h);
-    if (a.w_pre) {
-        float s = 0.0f, w[E];
+    load_channels<ALIGNED, E>(a.w_pre, a.pre_dtype, a.H, at, a.tpr, 0.0f, wn);
+    for (int64_t base = first; base < a.T; base += stride) {
+        const int64_t row = base + group;
+        const bool mine = row < a.T;
+        fetch(row + stride, next);
+        float h[E], inv1 = 1.0f, inv2 = 1.0f;
+        if (a.w_post) {
+            float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s = __fmaf_rn(h[e], h[e], s);
-        load_channels<N, E>(a.w_pre, a.pre_dtype, a.H, at, a.tpr, 0.0f, w);
-        row_sum<1>(&s, part[1], a.tpr);
-        inv2 = 1.0f / sqrtf(__fmaf_rn(s, inv_h, a.eps));
+            for (int e = 0; e < E; ++e) s = __fmaf_rn(cur.y.get(e), cur.y.get(e), s);
+            row_sum<1>(&s, part[0], a.tpr);
+            inv1 = 1.0f / sqrtf(__fmaf_rn(s, inv_h, a.eps));
+        }
+        const float factor = inv1 * cur.token;
 #pragma unroll
-        for (int e = 0; e < E; ++e) h[e] = h[e] * inv2 * w[e];
-        if (mine) store_share<TY, N, E>(n_out, row, a.H, at, a.tpr, h);
-    }
-    if (mine && stats && at == 0) {
-        stats[2 * row] = inv1;
-        stats[2 * row + 1] = inv2;
+        for (int e = 0; e < E; ++e) h[e] = a.y ? __fmaf_rn(w[e], cur.y.get(e) * factor, cur.r.get(e)) : cur.r.get(e);
+        if (mine && h_out) store_share<TR, ALIGNED, E>(h_out, row, a.H, at, a.tpr, h);
+        if (a.w_pre) {
+            float s = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) s = __fmaf_rn(h[e], h[e], s);
+            row_sum<1>(&s, part[1], a.tpr);
+            inv2 = 1.0f / sqrtf(__fmaf_rn(s, inv_h, a.eps));
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] = h[e] * inv2 * wn[e];
+            if (mine) store_share<TY, ALIGNED, E>(n_out, row, a.H, at, a.tpr, h);
+        }
+        if (!a.w_post || !a.w_pre) __syncthreads();          // one sum a row: its buffer is used again at once
+        if (mine && stats && at == 0) {
+            stats[2 * row] = inv1;
+            stats[2 * row + 1] = inv2;
+        }
+        cur = next;
     }
 }
 
@@ -193,40 +254,42 @@ struct NormGrad {
     int want_z, want_v;
 };
 
-template <int N, int E, bool WIDE>
+template <bool ALIGNED, int E, bool WIDE>
 __device__ __forceinline__ void take_channels(const void *v, int dtype, const float *lds, int64_t H, int at, int tpr,
                                               float fill, float *f) {
     if constexpr (WIDE) {
-        load_channels<N, E>(v, dtype, H, at, tpr, fill, f);
+        load_channels<ALIGNED, E>(v, dtype, H, at, tpr, fill, f);
     } else {
 #pragma unroll
-        for (int i = 0; i < E / N; ++i) {
-            const int c = (at + i * tpr) * N;
+        for (int i = 0; i < E / 8; ++i) {
+            const int c = (at + i * tpr) * 8;
 #pragma unroll
-            for (int j = 0; j < N; ++j) f[i * N + j] = fill;
-            if (v && c < H) {
+            for (int j = 0; j < 8; ++j) f[i * 8 + j] = fill;
+            if (v && c < H) {                                // whole pieces: the LDS rows are padded to them
 #pragma unroll
-                for (int j = 0; j < N; ++j) f[i * N + j] = lds[c + j];
+                for (int j = 0; j < 8; ++j) f[i * 8 + j] = lds[c + j];
             }
         }
     }
 }
 
-template <int TY, int TR, int N, int E, bool WIDE>
+template <int TY, int TR, bool ALIGNED, int E, bool WIDE>
 __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs a, NormGrad d) {
-    __shared__ float part[2][kNormThreads / kWave * 3];
-    extern __shared__ float vectors[];                       // [3][H]: w_post, gate per channel, w_pre
+    __shared__ float part[2][kNormWaves * 3];
+    extern __shared__ float vectors[];                       // [3][H up to a piece]: w_post, gate, w_pre
     const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / a.tpr);          // whole waves per row
     const int at = (int)threadIdx.x - group * a.tpr;
     const float inv_h = 1.0f / (float)a.H;
     const int64_t stride = (int64_t)gridDim.x * a.groups;
     const void *channel_gate = a.gate_kind == TERRACE_GATE_CHANNEL ? a.gate : nullptr;
-    float *lds_post = vectors, *lds_gate = vectors + a.H, *lds_pre = vectors + 2 * a.H;
+    const int padded = (int)((a.H + 7) / 8 * 8);
+    float *lds_post = vectors, *lds_gate = vectors + padded, *lds_pre = vectors + 2 * padded;
     if constexpr (!WIDE) {
-        for (int64_t c = threadIdx.x; c < a.H; c += blockDim.x) {
-            if (a.w_post) lds_post[c] = load_scalar(a.w_post, a.post_dtype, c);
-            if (channel_gate) lds_gate[c] = load_scalar(channel_gate, a.gate_dtype, c);
-            if (a.w_pre) lds_pre[c] = load_scalar(a.w_pre, a.pre_dtype, c);
+        for (int c = threadIdx.x; c < padded; c += blockDim.x) {
+            const bool in = c < a.H;
+            if (a.w_post) lds_post[c] = in ? load_scalar(a.w_post, a.post_dtype, c) : 0.0f;
+            if (channel_gate) lds_gate[c] = in ? load_scalar(channel_gate, a.gate_dtype, c) : 0.0f;
+            if (a.w_pre) lds_pre[c] = in ? load_scalar(a.w_pre, a.pre_dtype, c) : 0.0f;
         }
         __syncthreads();
     }
@@ -236,8 +299,8 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
         for (int e = 0; e < E; ++e) sum[0][e] = sum[1][e] = 0.0f;
     }
     struct Row {
-        Share<TY, N, E> y, dn;
-        Share<TR, N, E> r, dh;
+        Share<TY, ALIGNED, E> y, dn;
+        Share<TR, ALIGNED, E> r, dh;
         float inv1, inv2, token;
     };
     auto fetch = [&](int64_t row, Row &x) {
@@ -263,9 +326,9 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
         float s[3] = {0.0f, 0.0f, 0.0f};
         const float factor = a.scale * cur.token;            // scale, and the token's gate where there is one
         float wp[E], gc[E], wn[E];
-        take_channels<N, E, WIDE>(a.w_post, a.post_dtype, lds_post, a.H, at, a.tpr, 1.0f, wp);
-        take_channels<N, E, WIDE>(channel_gate, a.gate_dtype, lds_gate, a.H, at, a.tpr, 1.0f, gc);
-        take_channels<N, E, WIDE>(a.w_pre, a.pre_dtype, lds_pre, a.H, at, a.tpr, 0.0f, wn);
+        take_channels<ALIGNED, E, WIDE>(a.w_post, a.post_dtype, lds_post, a.H, at, a.tpr, 1.0f, wp);
+        take_channels<ALIGNED, E, WIDE>(channel_gate, a.gate_dtype, lds_gate, a.H, at, a.tpr, 1.0f, gc);
+        take_channels<ALIGNED, E, WIDE>(a.w_pre, a.pre_dtype, lds_pre, a.H, at, a.tpr, 0.0f, wn);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float u = cur.y.get(e) * cur.inv1, q = gc[e] * (u * wp[e]);
@@ -279,9 +342,9 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
         const float mean_tv = s[0] * inv_h;
         const float dot = __fmaf_rn(-cur.inv2 * mean_tv, s[2], s[1]);         // sum of dH * gate per channel * p
         const float mean_u = factor * dot * inv_h;
-        take_channels<N, E, WIDE>(a.w_post, a.post_dtype, lds_post, a.H, at, a.tpr, 1.0f, wp);
-        take_channels<N, E, WIDE>(channel_gate, a.gate_dtype, lds_gate, a.H, at, a.tpr, 1.0f, gc);
-        take_channels<N, E, WIDE>(a.w_pre, a.pre_dtype, lds_pre, a.H, at, a.tpr, 0.0f, wn);
+        take_channels<ALIGNED, E, WIDE>(a.w_post, a.post_dtype, lds_post, a.H, at, a.tpr, 1.0f, wp);
+        take_channels<ALIGNED, E, WIDE>(channel_gate, a.gate_dtype, lds_gate, a.H, at, a.tpr, 1.0f, gc);
+        take_channels<ALIGNED, E, WIDE>(a.w_pre, a.pre_dtype, lds_pre, a.H, at, a.tpr, 0.0f, wn);
         float o1[E], o2[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -297,7 +360,7 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
                 sum[0][e] = __fmaf_rn(z, u, sum[0][e]);
                 sum[1][e] = __fmaf_rn(dn, v, sum[1][e]);
             } else if (mine) {                               // one group: this lane alone touches the channel's cells
-                const int64_t c = ((int64_t)at + (int64_t)(e / N) * a.tpr) * N + e % N;
+                const int64_t c = ((int64_t)at + (int64_t)(e / 8) * a.tpr) * 8 + e % 8;
                 if (c < a.H) {
                     float *cell = d.partial + (int64_t)blockIdx.x * a.H + c;
                     if (d.want_z) *cell = base == first ? z * u : __fmaf_rn(z, u, *cell);
@@ -307,8 +370,8 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
             }
         }
         if (mine) {
-            if (d.d_residual) store_share<TR, N, E>(d.d_residual, row, a.H, at, a.tpr, o1);
-            if (d.dy) store_share<TY, N, E>(d.dy, row, a.H, at, a.tpr, o2);
+            if (d.d_residual) store_share<TR, ALIGNED, E>(d.d_residual, row, a.H, at, a.tpr, o1);
+            if (d.dy) store_share<TY, ALIGNED, E>(d.dy, row, a.H, at, a.tpr, o2);
             if (d.d_token && at == 0) {
                 const float dg = a.scale * dot;
                 if (a.gate_dtype == TERRACE_F32) store_floats<TERRACE_F32, 1>(d.d_token, row, &dg);
@@ -327,14 +390,14 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
             if (!want[k]) continue;
             float *out = d.partial + ((int64_t)k * gridDim.x + blockIdx.x) * a.H;
             if (a.groups == 1) {
-                store_share<TERRACE_F32, N, E>(out, 0, a.H, at, a.tpr, sum[k]);
+                store_share<TERRACE_F32, ALIGNED, E>(out, 0, a.H, at, a.tpr, sum[k]);
                 continue;
             }
             for (int g = 0; g < a.groups; ++g) {             // the row groups one after the other: a fixed order
                 if (group == g) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const int c = (at + (e / N) * a.tpr) * N + e % N;
+                        const int c = (at + (e / 8) * a.tpr) * 8 + e % 8;
                         if (c < a.H) vectors[c] = g ? vectors[c] + sum[k][e] : sum[k][e];
                     }
                 }
@@ -386,20 +449,24 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float *__restri
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-constexpr int64_t kNormMaxH = 2 * 8 * kNormThreads;          // 16 elements a lane, rows in vectors of 8
-constexpr int64_t kNormMaxOdd = 8 * kNormThreads;            // 8 elements a lane
-constexpr int kNormGradBlocks = 256;                         // one workgroup a CU
+constexpr int64_t kNormMaxH = 2 * 8 * kNormThreads;          // 16 elements a lane
+constexpr int kNormBlocks = 512;                             // forward: two workgroups a CU
+constexpr int kNormGradBlocks = 256;                         // gradient: one
 
 static bool norm_float(int d) { return d == TERRACE_F32 || d == TERRACE_BF16 || d == TERRACE_F16; }
 
-// 0 when the rows cannot be taken; else N * 100 + E
-static int norm_form(const NormArgs &a, uintptr_t bits) {
-    if (a.H % 8 == 0 && (bits & 15) == 0) return a.H <= kNormMaxOdd ? 808 : a.H <= kNormMaxH ? 816 : 0;
-    return a.H <= kNormMaxOdd ? 108 : 0;
+// Elements a lane holds, and whether the rows are whole pieces on 16-byte boundaries (otherwise any alignment their
+// elements have).
+struct NormForm {
+    int per;
+    bool aligned;
+};
+static NormForm norm_form(const NormArgs &a, uintptr_t bits) {
+    return {a.H <= kNormMaxH / 2 ? 8 : 16, a.H % 8 == 0 && (bits & 15) == 0};
 }
 
 static int norm_check(const NormArgs &a, int y_dtype, int r_dtype) {
-    if (a.T < 0 || a.H <= 0 || !norm_float(y_dtype) || !norm_float(r_dtype) ||
+    if (a.T < 0 || a.H <= 0 || a.H > kNormMaxH || !norm_float(y_dtype) || !norm_float(r_dtype) ||
         (r_dtype != y_dtype && r_dtype != TERRACE_F32) || a.gate_kind < TERRACE_GATE_NONE || a.gate_kind > TERRACE_GATE_TOKEN ||
         (a.T > 0 && (a.gate_kind != TERRACE_GATE_NONE) != (a.gate != nullptr)) || (a.w_post && !norm_float(a.post_dtype)) ||
         (a.gate && !norm_float(a.gate_dtype)) || (a.w_pre && !norm_float(a.pre_dtype)) || a.T >= ((int64_t)1 << 22) ||
@@ -408,10 +475,15 @@ static int norm_check(const NormArgs &a, int y_dtype, int r_dtype) {
     return TERRACE_OK;
 }
 
-static void norm_shape(NormArgs &a, int form) {
-    const int per = form % 100;
+static void norm_shape(NormArgs &a, int per) {
     a.tpr = (int)(((a.H + per - 1) / per + kWave - 1) / kWave * kWave);
     a.groups = 1;
+}
+
+// Rows a workgroup works on at a time: as many as it has threads for, but no more than leave every CU a workgroup.
+static void norm_groups(NormArgs &a) {
+    const int64_t most = kNormThreads / a.tpr, even = a.T / 256;
+    a.groups = (int)(even < 1 ? 1 : even < most ? even : most);
 }
 
 #define TERRACE_NORM_TYPES(CALL)                                                                  \
@@ -429,17 +501,18 @@ int run_block_norm(const void *y, int y_dtype, const void *residual, int r_dtype
     if (rc != TERRACE_OK) return rc;
     uintptr_t bits = (uintptr_t)y | (uintptr_t)residual | (uintptr_t)w_post | (uintptr_t)w_pre | (uintptr_t)h | (uintptr_t)n;
     if (gate_kind == TERRACE_GATE_CHANNEL) bits |= (uintptr_t)gate;
-    const int form = norm_form(a, bits);
-    if (!form) return TERRACE_EINVAL;
+    const NormForm form = norm_form(a, bits);
     if (T == 0) return TERRACE_OK;
     if (!residual || (y && !h) || (w_pre && !n)) return TERRACE_EINVAL;
-    norm_shape(a, form);
-    if (a.tpr < kBlock) a.groups = kBlock / a.tpr;
-    const unsigned grid = (unsigned)((T + a.groups - 1) / a.groups), threads = (unsigned)(a.tpr * a.groups);
-#define TERRACE_NORM(Y, R)                                                                          \
-    if (form == 808) block_norm_kernel<Y, R, 8, 8><<<grid, threads, 0, s>>>(a, h, n, stats);        \
-    else if (form == 816) block_norm_kernel<Y, R, 8, 16><<<grid, threads, 0, s>>>(a, h, n, stats);  \
-    else block_norm_kernel<Y, R, 1, 8><<<grid, threads, 0, s>>>(a, h, n, stats)
+    norm_shape(a, form.per);
+    norm_groups(a);
+    const int64_t need = (T + a.groups - 1) / a.groups;
+    const unsigned grid = (unsigned)(need < kNormBlocks ? need : kNormBlocks), threads = (unsigned)(a.tpr * a.groups);
+#define TERRACE_NORM(Y, R)                                                                                             \
+    if (form.aligned && form.per == 8) block_norm_kernel<Y, R, true, 8><<<grid, threads, 0, s>>>(a, h, n, stats);       \
+    else if (form.aligned) block_norm_kernel<Y, R, true, 16><<<grid, threads, 0, s>>>(a, h, n, stats);                  \
+    else if (form.per == 8) block_norm_kernel<Y, R, false, 8><<<grid, threads, 0, s>>>(a, h, n, stats);                 \
+    else block_norm_kernel<Y, R, false, 16><<<grid, threads, 0, s>>>(a, h, n, stats)
     TERRACE_NORM_TYPES(TERRACE_NORM)
 #undef TERRACE_NORM
     return check_launch();
@@ -469,8 +542,8 @@ int run_block_norm_grad(const void *y, int y_dtype, const void *residual, int r_
     uintptr_t bits = (uintptr_t)y | (uintptr_t)residual | (uintptr_t)w_post | (uintptr_t)w_pre | (uintptr_t)dh |
                      (uintptr_t)dn | (uintptr_t)dy | (uintptr_t)d_residual | (uintptr_t)ws;
     if (gate_kind == TERRACE_GATE_CHANNEL) bits |= (uintptr_t)gate;
-    const int form = norm_form(a, bits);
-    if (!form || ((uintptr_t)ws & 3)) return TERRACE_EINVAL;
+    const NormForm form = norm_form(a, bits);
+    if ((uintptr_t)ws & 15) return TERRACE_EINVAL;
     const bool channel_gate = gate_kind == TERRACE_GATE_CHANNEL;
     const NormReduce red{d_post, channel_gate ? d_gate : nullptr, d_pre};
     const bool want_z = red.d_post || red.d_gate, want_v = red.d_pre != nullptr, sums = want_z || want_v;
@@ -478,17 +551,18 @@ int run_block_norm_grad(const void *y, int y_dtype, const void *residual, int r_
     unsigned grid = 0;
     if (T > 0) {
         if (!residual || !stats) return TERRACE_EINVAL;
-        norm_shape(a, form);
-        if (form != 816) a.groups = kNormThreads / a.tpr;
+        norm_shape(a, form.per);
+        if (form.per == 8) norm_groups(a);
         grid = norm_grad_grid(T, a.groups);
         const NormGrad d{dh, dn, stats, dy, d_residual, gate_kind == TERRACE_GATE_TOKEN ? d_gate : nullptr, (float *)ws, want_z,
                          want_v};
         const unsigned threads = (unsigned)(a.tpr * a.groups);
-        const size_t lds = form == 816 ? 0 : (size_t)(3 * H) * sizeof(float);
-#define TERRACE_NORM(Y, R)                                                                            \
-    if (form == 808) block_norm_grad_kernel<Y, R, 8, 8, false><<<grid, threads, lds, s>>>(a, d);      \
-    else if (form == 816) block_norm_grad_kernel<Y, R, 8, 16, true><<<grid, threads, lds, s>>>(a, d); \
-    else block_norm_grad_kernel<Y, R, 1, 8, false><<<grid, threads, lds, s>>>(a, d)
+        const size_t lds = form.per == 16 ? 0 : (size_t)(3 * ((H + 7) / 8 * 8)) * sizeof(float);
+#define TERRACE_NORM(Y, R)                                                                                              \
+    if (form.aligned && form.per == 8) block_norm_grad_kernel<Y, R, true, 8, false><<<grid, threads, lds, s>>>(a, d);    \
+    else if (form.aligned) block_norm_grad_kernel<Y, R, true, 16, true><<<grid, threads, lds, s>>>(a, d);                \
+    else if (form.per == 8) block_norm_grad_kernel<Y, R, false, 8, false><<<grid, threads, lds, s>>>(a, d);              \
+    else block_norm_grad_kernel<Y, R, false, 16, true><<<grid, threads, lds, s>>>(a, d)
         TERRACE_NORM_TYPES(TERRACE_NORM)
 #undef TERRACE_NORM
     }

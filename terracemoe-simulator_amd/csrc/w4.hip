@@ -1,7 +1,7 @@
 // The experts' products for a few rows each, on 4-bit weights with group scales.
 //
-//   w4_pack_kernel    codes, scales and zero points into the order the product reads them (once per weight)
-//   w4_linear_kernel  out[i, n] = sum_k scale[e, n, k / g] * (code[e, n, k] - zero[e, n, k / g]) * x[i, k]
+//   w4_pack_*_kernel                codes, scales and zero points into the order the product reads them (once per weight)
+//   w4_few_kernel, w4_many_kernel   out[i, n] = sum_k scale[e, n, k / g] * (code[e, n, k] - zero[e, n, k / g]) * x[i, k]
 //                     for the rows i of expert e; optionally silu(first half of the columns) * (second half)
 //
 // Few rows per expert, so the product reads every code once and does little with it: it is bound by the HBM bytes of
@@ -23,7 +23,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // takes from that lane, so a wave's load of a block is one contiguous kilobyte and any group of 32, 64 or 128 ends
 // with an instruction.  Inside a dword code 2i sits in nibble i and code 2i + 1 in nibble i + 4, 16 bits apart, so that one
 // shift and one mask leave a pair of neighbouring codes in the two halves of a register.  Scales and zero points:
-// [experts][column tiles][groups, up to a whole block][16 columns].  Columns past N and k past K hold zeros.
+// [experts][column tiles][blocks][16 columns][groups of a block], so a lane has those of a block in one load.  Columns
+// past N and k past K hold zeros.
 constexpr int kTileN = 16, kBlockK = 128;
 
 struct W4Shape {
@@ -35,7 +36,8 @@ struct W4Shape {
     __host__ __device__ int64_t groups() const { return blocks() * (kBlockK / group); }
     bool ok() const {
         return n_experts > 0 && n_experts <= (1 << 20) && N > 0 && K > 0 && N <= (1 << 24) && K <= (1 << 24) &&
-               (group == 32 || group == 64 || group == 128) && K % group == 0;
+               (group == 32 || group == 64 || group == 128) && K % group == 0 &&
+               tiles() * blocks() < (1 << 21);               // an expert's codes stay below 2^31 bytes: 32-bit offsets
     }
 };
 
@@ -68,10 +70,13 @@ __global__ __launch_bounds__(kBlock) void w4_pack_groups_kernel(const V *__restr
                                                                 V *__restrict__ packed, int64_t total) {
     const int64_t step = (int64_t)gridDim.x * kBlock, groups = sh.K / sh.group;
     for (int64_t d = (int64_t)blockIdx.x * kBlock + threadIdx.x; d < total; d += step) {
-        int64_t rest = d / kTileN;
-        const int64_t g = rest % sh.groups();
-        rest /= sh.groups();
-        const int64_t n = rest % sh.tiles() * kTileN + d % kTileN, e = rest / sh.tiles();
+        const int gpb = kBlockK / sh.group;
+        int64_t rest = d / gpb;
+        const int64_t col = rest % kTileN;
+        rest /= kTileN;
+        const int64_t g = rest % sh.blocks() * gpb + d % gpb;
+        rest /= sh.blocks();
+        const int64_t n = rest % sh.tiles() * kTileN + col, e = rest / sh.tiles();
         packed[d] = n < sh.N && g < groups ? plane[(e * sh.N + n) * groups + g] : V(0);
     }
 }
@@ -145,248 +150,403 @@ __device__ __forceinline__ typename W4Type<DT>::Frag w4_expand(uint32_t w) {
     return __builtin_bit_cast(typename W4Type<DT>::Frag, v);
 }
 
-// Which expert's rows a row tile holds.  Tiles of R rows are counted expert by expert; every wave finds its own by a scan
-// over the counts, 64 lanes holding `per` consecutive experts each.  Counts are the caller's device data: each is taken
-// into [0, P] and the sums saturate at P, so no count names a row outside the P rows.
+// Which expert's rows a row tile holds.  Tiles of R rows are counted expert by expert; every wave finds its own by scans
+// over the counts, a lane an expert, 64 at a time.  Counts are the caller's device data: each is taken into [0, P] and the
+// sums saturate at P, so no count names a row outside the P rows.
 struct RowTile {
     int expert;       // -1: past the last tile
     int first, rows;  // its rows
-    int tiles, live;  // tiles and rows in all
+    int tiles, live;  // past the last tile only: tiles and rows in all
 };
 
+// Inclusive scan over the wave, every sum cut at `most` (all values in [0, most], most <= 2^30).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v, int most) {
+    const int t = v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+    return t < most ? t : most;
+}
+__device__ __forceinline__ int wave_scan(int v, int most) {
+    v = scan_step<0x111, 0xF>(v, most);                      // row_shr:1, 2, 4, 8 inside the rows of 16 lanes
+    v = scan_step<0x112, 0xF>(v, most);
+    v = scan_step<0x114, 0xF>(v, most);
+    v = scan_step<0x118, 0xF>(v, most);
+    v = scan_step<0x142, 0xA>(v, most);                      // and the rows' totals upwards
+    return scan_step<0x143, 0xC>(v, most);
+}
+
 __device__ __forceinline__ RowTile find_tile(const int64_t *__restrict__ counts, int n_experts, int P, int R, int tile) {
-    const int lane = lane_id(), per = (n_experts + kWave - 1) / kWave, e0 = lane * per;
-    int my_rows = 0, my_tiles = 0;
-    for (int i = 0; i < per; ++i) {
-        const int64_t c = e0 + i >= n_experts ? 0 : counts ? counts[e0 + i] : P;
-        int n = c < 0 ? 0 : c > P ? P : (int)c;
-        n = n < P - my_rows ? n : P - my_rows;
-        my_rows += n;
-        my_tiles += (n + R - 1) / R;
-    }
-    int rows = my_rows;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int r = __shfl_up(rows, d, kWave);
-        if (lane >= d) rows = rows + r < P ? rows + r : P;
-    }
-    // a lane whose rows saturate keeps what is left for it; its tiles may then be fewer than it counted
-    int before = __shfl_up(rows, 1, kWave);
-    if (lane == 0) before = 0;
-    if (rows - before < my_rows) {
-        int left = rows - before;
-        my_tiles = 0;
-        for (int i = 0; i < per; ++i) {
-            const int64_t c = e0 + i >= n_experts ? 0 : counts ? counts[e0 + i] : P;
-            int n = c < 0 ? 0 : c > left ? left : (int)c;
-            left -= n;
-            my_tiles += (n + R - 1) / R;
+    const int lane = lane_id();
+    int rows = 0, tiles = 0;                                 // before the experts looked at
+    auto count = [&](int e) { return e >= n_experts ? (int64_t)0 : counts ? counts[e] : (int64_t)P; };
+    int64_t c = count(lane);
+    for (int e0 = 0; e0 < n_experts; e0 += kWave) {
+        const int64_t now = c;
+        c = count(e0 + kWave + lane);
+        const int n = now < 0 ? 0 : now > P ? P : (int)now;
+        int upto = wave_scan(n, P) + rows;
+        if (upto > P) upto = P;
+        int from = __shfl_up(upto, 1, kWave);
+        if (lane == 0) from = rows;
+        const int mine = (upto - from + R - 1) / R;
+        const int upto_tiles = wave_scan(mine, P) + tiles;
+        const uint64_t past = __ballot(upto_tiles > tile);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            const int skip = (tile - read_lane(upto_tiles - mine, at)) * R;
+            const int first = read_lane(from, at), n_rows = read_lane(upto, at) - first - skip;
+            return {e0 + at, first + skip, n_rows < R ? n_rows : R, 0, 0};
         }
+        rows = read_lane(upto, kWave - 1);
+        tiles = read_lane(upto_tiles, kWave - 1);
     }
-    int upto = my_tiles;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int t = __shfl_up(upto, d, kWave);
-        if (lane >= d) upto += t;
-    }
-    RowTile out;
-    out.tiles = __shfl(upto, kWave - 1, kWave);
-    out.live = __shfl(rows, kWave - 1, kWave);
-    out.expert = -1;
-    out.first = out.rows = 0;
-    const uint64_t past = __ballot(upto > tile);
-    if (past == 0) return out;
-    // the owning lane walks its own experts
-    if (lane == __builtin_ctzll(past)) {
-        int t = upto - my_tiles, r = before;
-        for (int i = 0; i < per; ++i) {
-            const int64_t c = e0 + i >= n_experts ? 0 : counts ? counts[e0 + i] : P;
-            const int n = c < 0 ? 0 : c > rows - r ? rows - r : (int)c;
-            const int nt = (n + R - 1) / R;
-            if (tile < t + nt) {
-                const int skip = (tile - t) * R;
-                out.expert = e0 + i;
-                out.first = r + skip;
-                out.rows = n - skip < R ? n - skip : R;
-                break;
-            }
-            t += nt;
-            r += n;
-        }
-    }
-    const int owner = __builtin_ctzll(past);
-    out.expert = read_lane(out.expert, owner);
-    out.first = read_lane(out.first, owner);
-    out.rows = read_lane(out.rows, owner);
-    return out;
+    return {-1, 0, 0, tiles, rows};
 }
 
 struct W4Args {
     const void *x;
-    const int64_t *counts;
+    const int64_t *counts;     // NULL: one expert with all rows
     int P;
     W4Shape sh;
     const u32x4 *codes;
     const uint16_t *scales;
     const uint8_t *zeros;      // NULL: 8
     int swiglu;
-    int col_groups;            // workgroups along the columns
     void *out;
+    // worked out once on the host
+    int out_cols;
+    int tiles, blocks;         // column tiles of the weights and packed blocks of k
+    int full, rest;            // whole blocks of k, and the steps of 32 in what is left
+    int col_blocks;            // workgroups along the columns
+    int split, per;            // few rows: waves that share out the k of one set of columns, and the whole blocks of each
+    int sets;                  // few rows: sets of columns in a workgroup
 };
 
-// A workgroup makes 32 columns -- two tiles: neighbours, or with `swiglu` the same columns of both halves -- of up to 16 * MT
-// rows of one expert.  Its waves share out the blocks of k and are joined in LDS, in order.  GS: matrix steps per group.
-constexpr int w4_max_waves(int mt) { return mt == 1 ? 8 : 4; }
+// Rows no expert owns are zeros; the workgroups past the last tile write the columns [lo, hi) of them.
+__device__ __forceinline__ void w4_zero_rows(const W4Args &a, const RowTile &rt, int tile, int lo, int hi) {
+    const int spare = (int)(gridDim.x / (unsigned)a.col_blocks) - rt.tiles;
+    if (hi > a.out_cols) hi = a.out_cols;
+    for (int64_t r = rt.live + (tile - rt.tiles); r < a.P; r += spare)
+        for (int c = lo + (int)threadIdx.x; c < hi; c += (int)blockDim.x) ((uint16_t *)a.out)[r * a.out_cols + c] = 0;
+}
 
-template <int DT, int MT, int GS>
-__global__ __launch_bounds__(w4_max_waves(MT) * kWave) void w4_linear_kernel(W4Args a) {
-    typedef typename W4Type<DT>::Frag Frag;
-    extern __shared__ float lds[];
-    constexpr int R = 16 * MT;
-    const int lane = lane_id(), w = wave_in_block(), waves = (int)(blockDim.x >> 6);
-    const int cg = (int)(blockIdx.x % (unsigned)a.col_groups), tile = (int)(blockIdx.x / (unsigned)a.col_groups);
-    const int grid_tiles = (int)(gridDim.x / (unsigned)a.col_groups);
-    const int64_t N = a.sh.N, K = a.sh.K, out_cols = a.swiglu ? N / 2 : N;
-    const RowTile rt = find_tile(a.counts, a.sh.n_experts, a.P, R, tile);
-    const int c16 = lane & 15, q = lane >> 4;
-    // the two columns of this lane
-    const int64_t col0 = a.swiglu ? 16 * (int64_t)cg + c16 : 32 * (int64_t)cg + c16;
-    const int64_t col1 = a.swiglu ? col0 + N / 2 : col0 + 16;
-    uint16_t *out = (uint16_t *)a.out;
-    if (rt.expert < 0) {                                     // rows no expert owns are zeros; the spare tiles write them
-        for (int64_t r = rt.live + (tile - rt.tiles); r < a.P; r += grid_tiles - rt.tiles) {
-            if (threadIdx.x < 16) {
-                if (col0 < out_cols) out[r * out_cols + col0] = 0;
-                if (!a.swiglu && col1 < out_cols) out[r * out_cols + col1] = 0;
-            }
-        }
-        return;
-    }
-    const int64_t blocks = a.sh.blocks(), tiles = a.sh.tiles();
-    const int64_t per = (blocks + waves - 1) / waves, b0 = w * per, b1 = b0 + per < blocks ? b0 + per : blocks;
-    const int64_t n0 = col0 < N ? col0 : N - 1, n1 = col1 < N ? col1 : N - 1;      // in bounds; dropped at the store
-    const int64_t t0 = (int64_t)rt.expert * tiles + n0 / 16, t1 = (int64_t)rt.expert * tiles + n1 / 16;
-    const u32x4 *w0 = a.codes + t0 * blocks * kWave + q * 16 + n0 % 16;
-    const u32x4 *w1 = a.codes + t1 * blocks * kWave + q * 16 + n1 % 16;
-    constexpr int GPB = 4 / GS;                              // groups per block
-    const int64_t s0 = t0 * a.sh.groups() * kTileN + n0 % 16, s1 = t1 * a.sh.groups() * kTileN + n1 % 16;
-    const uint16_t *xr[MT];
-    bool has[MT];
+// A lane's column of one expert: byte offsets of its codes and (in groups) of its scales from the expert's first.
+struct W4Expert {
+    const uint8_t *codes, *scales, *zeros;                   // of the tile's expert; zeros may be NULL
+};
+struct W4Column {
+    uint32_t codes, groups;
+};
+__device__ __forceinline__ W4Expert w4_expert(const W4Args &a, int expert, int gpb) {
+    const int64_t blocks = (int64_t)expert * a.tiles * a.blocks, groups = blocks * (gpb * kTileN);
+    return {(const uint8_t *)a.codes + blocks * 1024, (const uint8_t *)a.scales + 2 * groups,
+            a.zeros ? a.zeros + groups : nullptr};
+}
+__device__ __forceinline__ W4Column w4_column(const W4Args &a, int col, int q, int gpb) {
+    const uint32_t n = (uint32_t)(col < (int)a.sh.N ? col : (int)a.sh.N - 1);      // in bounds; dropped at the store
+    const uint32_t block = n / kTileN * (uint32_t)a.blocks;
+    return {block * 1024u + (uint32_t)(q * 16 + n % kTileN) * 16u, (block * kTileN + n % kTileN) * gpb};
+}
+
+// T tiles of a block of k: codes, scales and zero points of this lane's columns.
+template <int GPB>
+struct GroupBits;
+template <>
+struct GroupBits<1> { typedef uint16_t S; typedef uint8_t Z; };
+template <>
+struct GroupBits<2> { typedef uint32_t S; typedef uint16_t Z; };
+template <>
+struct GroupBits<4> { typedef u32x2 S; typedef uint32_t Z; };
+template <int T, int GPB, bool ZEROS>
+struct W4Block {
+    u32x4 w[T];
+    static constexpr int kWords = GPB == 4 ? 2 : 1;
+    uint32_t s[T][kWords];                                   // a scale in each half
+    uint32_t z[T];                                           // a zero point in each byte
+    __device__ __forceinline__ void fetch(const W4Expert &e, const W4Column *col, int b) {
+        const uint8_t *codes = e.codes + (int64_t)b * 1024, *scales = e.scales + (int64_t)b * (2 * GPB * kTileN);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        has[m] = 16 * m + c16 < rt.rows;
-        xr[m] = (const uint16_t *)a.x + (int64_t)(rt.first + (has[m] ? 16 * m + c16 : 0)) * K + 8 * q;
+        for (int t = 0; t < T; ++t) {
+            w[t] = *(const u32x4 *)(codes + col[t].codes);
+            const auto v = *(const typename GroupBits<GPB>::S *)(scales + 2u * col[t].groups);
+            if constexpr (GPB == 4) s[t][0] = v[0], s[t][1] = v[1];
+            else s[t][0] = v;
+        }
+        if constexpr (ZEROS) {
+            const uint8_t *zeros = e.zeros + (int64_t)b * (GPB * kTileN);
+#pragma unroll
+            for (int t = 0; t < T; ++t) z[t] = *(const typename GroupBits<GPB>::Z *)(zeros + col[t].groups);
+        } else {
+#pragma unroll
+            for (int t = 0; t < T; ++t) z[t] = 0x08080808u;
+        }
     }
+};
+
+// total += the block's products: x(m, s) gives the rows' fragment of step s.
+template <int DT, int MT, int T, int GS, bool ZEROS, typename X>
+__device__ __forceinline__ void w4_use(W4Block<T, 4 / GS, ZEROS> &k, X x, f32x4 (*total)[T]) {
+    typedef typename W4Type<DT>::Frag Frag;
     const u32x4 ones4 = {W4Type<DT>::kOnes, W4Type<DT>::kOnes, W4Type<DT>::kOnes, W4Type<DT>::kOnes};
     const Frag ones = __builtin_bit_cast(Frag, ones4);
-    f32x4 total[MT][2];
+    // what was fetched stays as it came until here: without this the compiler unpacks it where it arrives, and a ring of
+    // unpacked blocks does not fit the registers
 #pragma unroll
-    for (int m = 0; m < MT; ++m) total[m][0] = total[m][1] = f32x4{0, 0, 0, 0};
+    for (int t = 0; t < T; ++t) {
+        asm volatile("" : "+v"(k.w[t]), "+v"(k.z[t]));
+#pragma unroll
+        for (int i = 0; i < W4Block<T, 4 / GS, ZEROS>::kWords; ++i) asm volatile("" : "+v"(k.s[t][i]));
+    }
+    f32x4 acc[MT][T], sum[MT];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const f32x4 zero = {0, 0, 0, 0};
+        const bool first = s % GS == 0;
+        Frag xs[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            xs[m] = __builtin_bit_cast(Frag, x(m, s));
+            sum[m] = W4Type<DT>::mfma(xs[m], ones, first ? zero : sum[m]);
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const Frag f = w4_expand<DT>(k.w[t][s]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m][t] = W4Type<DT>::mfma(xs[m], f, first ? zero : acc[m][t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);                   // one step's expanded codes at a time in registers
+        if (s % GS != GS - 1) continue;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            float scale;
+            const int g = s / GS;
+            const uint32_t bits = g & 1 ? k.s[t][g / 2] >> 16 : k.s[t][g / 2] & 0xFFFFu;
+            if constexpr (DT == TERRACE_BF16) scale = bf16_bits_to_f32(bits);
+            else scale = __half2float(__ushort_as_half((unsigned short)bits));
+            const float off = -16.0f - (float)((k.z[t] >> (8 * g)) & 0xFFu);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    total[m][t][i] = __fmaf_rn(scale, __fmaf_rn(off, sum[m][i], acc[m][t][i]), total[m][t][i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
 
+__device__ __forceinline__ float w4_swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+
+// Few rows: tiles of 16.  A set of 32 columns -- two tiles: neighbours, or with `swiglu` the same columns of both halves --
+// is the work of `split` waves that share out the blocks of k and are joined in LDS, in order; a workgroup holds 4 or 8
+// waves and so 4 / split or 8 / split sets.  The rows' fragments come straight from memory (a few rows: L1 and L2), and
+// codes and rows are fetched kAhead blocks ahead, because the codes come from HBM and nothing else hides their latency.
+constexpr int kAhead = 3;
+constexpr int kMaxSplit = 8;
+
+template <int DT, int GS, bool ZEROS>
+__global__ __launch_bounds__(kMaxSplit * kWave) __attribute__((amdgpu_waves_per_eu(4))) void w4_few_kernel(W4Args a) {
+    __shared__ float lds[kMaxSplit][8][kWave];
+    const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_in_block());
+    const int cb = (int)(blockIdx.x % (unsigned)a.col_blocks), tile = (int)(blockIdx.x / (unsigned)a.col_blocks);
+    const int width = a.swiglu ? 16 : 32, lo = cb * a.sets * width;
+    const RowTile rt = find_tile(a.counts, a.sh.n_experts, a.P, 16, tile);
+    if (rt.expert < 0) {
+        w4_zero_rows(a, rt, tile, lo, lo + a.sets * width);
+        return;
+    }
+    const int c16 = lane & 15, q = lane >> 4, set = w / a.split, part = w - set * a.split;
+    const int col0 = lo + set * width + c16, col1 = a.swiglu ? col0 + a.out_cols : col0 + 16;
+    const W4Expert we = w4_expert(a, rt.expert, 4 / GS);
+    const W4Column col[2] = {w4_column(a, col0, q, 4 / GS), w4_column(a, col1, q, 4 / GS)};
+    const int b0 = part * a.per < a.full ? part * a.per : a.full, b1 = b0 + a.per < a.full ? b0 + a.per : a.full;
+    // a lane without a row reads the tile's first one: the same lines, and its results are dropped
+    const uint8_t *xt = (const uint8_t *)a.x + (int64_t)rt.first * a.sh.K * 2;
+    const uint32_t xo = (uint32_t)((c16 < rt.rows ? c16 : 0) * (int)a.sh.K + 8 * q) * 2u;
+    f32x4 total[1][2] = {{f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}};
     struct Block {
-        u32x4 w[2];
-        u32x4 x[MT][4];
-        uint16_t s[2][GPB];
-        uint8_t z[2][GPB];
+        W4Block<2, 4 / GS, ZEROS> k;
+        u32x4 x[4];
     };
-    auto fetch = [&](int64_t b, Block &k) {
-        k.w[0] = w0[b * kWave];
-        k.w[1] = w1[b * kWave];
+    auto fetch = [&](int b, Block &f) {
+        f.k.fetch(we, col, b);
+        const uint8_t *xb = xt + (int64_t)b * (2 * kBlockK);
 #pragma unroll
-        for (int g = 0; g < GPB; ++g) {
-            k.s[0][g] = a.scales[s0 + (b * GPB + g) * kTileN];
-            k.s[1][g] = a.scales[s1 + (b * GPB + g) * kTileN];
-            k.z[0][g] = k.z[1][g] = 8;
-            if (a.zeros) {
-                k.z[0][g] = a.zeros[s0 + (b * GPB + g) * kTileN];
-                k.z[1][g] = a.zeros[s1 + (b * GPB + g) * kTileN];
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int64_t at = b * kBlockK + 32 * s;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                k.x[m][s] = zero_of<u32x4>();
-                if (has[m] && at < K) k.x[m][s] = *(const u32x4 *)(xr[m] + at);
-            }
-        }
+        for (int s = 0; s < 4; ++s) f.x[s] = *(const u32x4 *)(xb + xo + 64 * s);
     };
-    auto use = [&](const Block &k) {
-        f32x4 acc[MT][2], sum[MT];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const Frag f0 = w4_expand<DT>(k.w[0][s]), f1 = w4_expand<DT>(k.w[1][s]);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const Frag x = __builtin_bit_cast(Frag, k.x[m][s]);
-                const f32x4 zero = {0, 0, 0, 0};
-                const bool first = s % GS == 0;
-                acc[m][0] = W4Type<DT>::mfma(x, f0, first ? zero : acc[m][0]);
-                acc[m][1] = W4Type<DT>::mfma(x, f1, first ? zero : acc[m][1]);
-                sum[m] = W4Type<DT>::mfma(x, ones, first ? zero : sum[m]);
-            }
-            if (s % GS == GS - 1) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    float scale;
-                    const uint16_t bits = k.s[t][s / GS];
-                    if constexpr (DT == TERRACE_BF16) scale = bf16_bits_to_f32(bits);
-                    else scale = __half2float(__ushort_as_half(bits));
-                    const float off = -(16.0f + (float)k.z[t][s / GS]);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            total[m][t][i] = __fmaf_rn(scale, __fmaf_rn(off, sum[m][i], acc[m][t][i]), total[m][t][i]);
-                }
-            }
-        }
+    auto use = [&](Block &f) {
+        w4_use<DT, 1, 2, GS, ZEROS>(f.k, [&](int, int s) { return f.x[s]; }, total);
     };
     if (b0 < b1) {
-        Block cur, next;
-        fetch(b0, cur);
-        for (int64_t b = b0; b < b1; ++b) {
-            if (b + 1 < b1) fetch(b + 1, next);
-            use(cur);
-            cur = next;
+        Block ring[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) fetch(b0 + i < b1 ? b0 + i : b1 - 1, ring[i]);
+        for (int b = b0; b < b1; b += kAhead) {              // past the end the last block is fetched again, from cache
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (b + i < b1) use(ring[i]);
+                fetch(b + kAhead + i < b1 ? b + kAhead + i : b1 - 1, ring[i]);
+            }
         }
     }
-    // join the waves: lds[w][m][t][i][lane]
-    constexpr int kPer = MT * 2 * 4;
+    if (a.rest && part == a.split - 1) {                     // a K that is no multiple of 128: zeros past it
+        Block f;
+        f.k.fetch(we, col, a.full);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            f.x[s] = zero_of<u32x4>();
+            if (s < a.rest) f.x[s] = *(const u32x4 *)(xt + (int64_t)a.full * (2 * kBlockK) + xo + 64 * s);
+        }
+        use(f);
+    }
+    auto store = [&](int i, float v0, float v1) {            // row i of this lane's quarter
+        const int row = 4 * q + i;
+        if (row >= rt.rows) return;
+        uint16_t *o = (uint16_t *)a.out + (int64_t)(rt.first + row) * a.out_cols;
+        if (a.swiglu) {
+            if (col0 < a.out_cols) o[col0] = (uint16_t)to_bits16<DT>(w4_swiglu(v0, v1));
+        } else {
+            if (col0 < a.out_cols) o[col0] = (uint16_t)to_bits16<DT>(v0);
+            if (col1 < a.out_cols) o[col1] = (uint16_t)to_bits16<DT>(v1);
+        }
+    };
+    if (a.split == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store(i, total[0][0][i], total[0][1][i]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        lds[w][i][lane] = total[0][0][i];
+        lds[w][4 + i][lane] = total[0][1][i];
+    }
+    __syncthreads();
+    for (int i = part; i < 4; i += a.split) {
+        float v0 = 0.0f, v1 = 0.0f;
+        for (int y = w - part; y < w - part + a.split; ++y) {
+            v0 += lds[y][i][lane];
+            v1 += lds[y][4 + i][lane];
+        }
+        store(i, v0, v1);
+    }
+}
+
+// Tens of rows: tiles of 16 * MT.  A workgroup of four waves makes 256 columns, each wave four tiles (with `swiglu` two of
+// each half), so the rows of a block of k are read once for 256 columns: they go through LDS in the order the matrix
+// instructions take them, one block ahead, while every wave streams its own codes two blocks ahead.
+template <int DT, int MT, int GS, bool ZEROS>
+__global__ __launch_bounds__(4 * kWave) void w4_many_kernel(W4Args a) {
+    constexpr int R = 16 * MT, T = 4;
+    __shared__ u32x4 rows[2][4][MT][kWave];                  // [buffer][step][16 rows][lane]
+    const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_in_block());
+    const int cb = (int)(blockIdx.x % (unsigned)a.col_blocks), tile = (int)(blockIdx.x / (unsigned)a.col_blocks);
+    const int width = a.swiglu ? 32 : 64, lo = cb * 4 * width;
+    const RowTile rt = find_tile(a.counts, a.sh.n_experts, a.P, R, tile);
+    if (rt.expert < 0) {
+        w4_zero_rows(a, rt, tile, lo, lo + 4 * width);
+        return;
+    }
+    const int c16 = lane & 15, q = lane >> 4;
+    const W4Expert we = w4_expert(a, rt.expert, 4 / GS);
+    int at[T];
+    W4Column col[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {                            // swiglu: tiles 0 and 2 of the first half, 1 and 3 their partners
+        at[t] = lo + w * width + c16 + (a.swiglu ? (t >> 1) * 16 + (t & 1) * a.out_cols : t * 16);
+        col[t] = w4_column(a, at[t], q, 4 / GS);
+    }
+    // wave w brings step w of a block: rows past the tile's last repeat it (their results are dropped)
+    const uint8_t *xt = (const uint8_t *)a.x + (int64_t)rt.first * a.sh.K * 2;
+    uint32_t xo[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int r = 16 * m + c16 < rt.rows ? 16 * m + c16 : rt.rows - 1;
+        xo[m] = (uint32_t)(r * (int)a.sh.K + 32 * w + 8 * q) * 2u;
+    }
+    const int blocks = a.blocks;
+    u32x4 xn[MT];
+    auto bring = [&](int b) {                                // the next block, or the last once more; zeros past K
+        const int c = b < blocks ? b : blocks - 1;
+        const bool in = c < a.full || w < a.rest;
+        const uint8_t *xb = xt + (int64_t)(in ? c : 0) * (2 * kBlockK);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) xn[m] = in ? *(const u32x4 *)(xb + xo[m]) : zero_of<u32x4>();
+    };
+    auto place = [&](int buf) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) rows[buf][w][m][lane] = xn[m];
+    };
+    f32x4 total[MT][T];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) lds[((w * MT + m) * 8 + t * 4 + i) * kWave + lane] = total[m][t][i];
+        for (int t = 0; t < T; ++t) total[m][t] = f32x4{0, 0, 0, 0};
+    W4Block<T, 4 / GS, ZEROS> ring[2];
+    ring[0].fetch(we, col, 0);
+    ring[1].fetch(we, col, blocks > 1 ? 1 : 0);
+    bring(0);
+    place(0);
     __syncthreads();
-    for (int j = w; j < MT * 4; j += waves) {                // row (m, i) of each lane's quarter, both columns
-        const int m = j >> 2, i = j & 3;
-        float v[2] = {0.0f, 0.0f};
-        for (int x = 0; x < waves; ++x) {
-            v[0] += lds[(x * kPer + m * 8 + i) * kWave + lane];
-            v[1] += lds[(x * kPer + m * 8 + 4 + i) * kWave + lane];
+    for (int b = 0; b < blocks; b += 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            bring(b + i + 1);
+            if (b + i < blocks)
+                w4_use<DT, MT, T, GS, ZEROS>(ring[i], [&](int m, int s) { return rows[i][s][m][lane]; }, total);
+            ring[i].fetch(we, col, b + i + 2 < blocks ? b + i + 2 : blocks - 1);
+            place(1 - i);
+            __syncthreads();
         }
-        const int row = 16 * m + 4 * q + i;
-        if (row >= rt.rows) continue;
-        uint16_t *o = out + (int64_t)(rt.first + row) * out_cols;
-        if (a.swiglu) {
-            const float y = v[0] / (1.0f + __expf(-v[0])) * v[1];
-            if (col0 < out_cols) o[col0] = (uint16_t)to_bits16<DT>(y);
-        } else {
-            if (col0 < out_cols) o[col0] = (uint16_t)to_bits16<DT>(v[0]);
-            if (col1 < out_cols) o[col1] = (uint16_t)to_bits16<DT>(v[1]);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 16 * m + 4 * q + i;
+            if (row >= rt.rows) continue;
+            uint16_t *o = (uint16_t *)a.out + (int64_t)(rt.first + row) * a.out_cols;
+            if (a.swiglu) {
+#pragma unroll
+                for (int t = 0; t < T; t += 2)
+                    if (at[t] < a.out_cols) o[at[t]] = (uint16_t)to_bits16<DT>(w4_swiglu(total[m][t][i], total[m][t + 1][i]));
+            } else {
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+                    if (at[t] < a.out_cols) o[at[t]] = (uint16_t)to_bits16<DT>(total[m][t][i]);
+            }
         }
     }
 }
 
-template <int DT, int MT>
-static void launch_w4_g(const W4Args &a, unsigned grid, int waves, hipStream_t s) {
-    const size_t lds = (size_t)waves * MT * 8 * kWave * sizeof(float);
-    if (a.sh.group == 128) w4_linear_kernel<DT, MT, 4><<<grid, waves * kWave, lds, s>>>(a);
-    else if (a.sh.group == 64) w4_linear_kernel<DT, MT, 2><<<grid, waves * kWave, lds, s>>>(a);
-    else w4_linear_kernel<DT, MT, 1><<<grid, waves * kWave, lds, s>>>(a);
+template <int DT, bool ZEROS>
+static void launch_w4(W4Args a, int64_t busy, hipStream_t s) {
+    const int64_t P = a.P;
+    // row tiles: the most there can be, and one for rows without an expert
+    auto tiles = [&](int64_t R) { return busy + (P - busy) / R + 1; };
+    const int64_t mean = (P + busy - 1) / busy;
+    const int mt = mean <= 32 ? 2 : 4;
+    const int64_t wide = a.swiglu ? (a.out_cols + 127) / 128 : (a.out_cols + 255) / 256;
+    if (mean > 16 && wide * (tiles(16 * mt) - 1) >= 256) {
+        a.col_blocks = (int)wide;
+        const unsigned grid = (unsigned)(wide * tiles(16 * mt));
+#define TERRACE_MANY(MT)                                                                            \
+    if (a.sh.group == 128) w4_many_kernel<DT, MT, 4, ZEROS><<<grid, 4 * kWave, 0, s>>>(a);          \
+    else if (a.sh.group == 64) w4_many_kernel<DT, MT, 2, ZEROS><<<grid, 4 * kWave, 0, s>>>(a);      \
+    else w4_many_kernel<DT, MT, 1, ZEROS><<<grid, 4 * kWave, 0, s>>>(a)
+        if (mt == 2) { TERRACE_MANY(2); }
+        else { TERRACE_MANY(4); }
+#undef TERRACE_MANY
+        return;
+    }
+    const int64_t sets = a.swiglu ? (a.out_cols + 15) / 16 : (a.out_cols + 31) / 32, n = sets * (tiles(16) - 1);
+    a.split = 1;
+    while (a.split < kMaxSplit && n * a.split < 4096 && a.full >= 2 * a.split) a.split *= 2;
+    const int waves = a.split > 4 ? a.split : 4;
+    a.per = (a.full + a.split - 1) / a.split;
+    a.sets = waves / a.split;
+    a.col_blocks = (int)((sets + a.sets - 1) / a.sets);
+    const unsigned grid = (unsigned)(a.col_blocks * tiles(16)), threads = (unsigned)(waves * kWave);
+    if (a.sh.group == 128) w4_few_kernel<DT, 4, ZEROS><<<grid, threads, 0, s>>>(a);
+    else if (a.sh.group == 64) w4_few_kernel<DT, 2, ZEROS><<<grid, threads, 0, s>>>(a);
+    else w4_few_kernel<DT, 1, ZEROS><<<grid, threads, 0, s>>>(a);
 }
 
 int run_w4_linear(const void *x, int dtype, int64_t P, const int64_t *counts, const void *codes, const void *scales,
@@ -397,24 +557,18 @@ int run_w4_linear(const void *x, int dtype, int64_t P, const int64_t *counts, co
         return TERRACE_EINVAL;
     if (P == 0) return TERRACE_OK;
     if (!x || (!counts && n_experts != 1) || !codes || !scales || !out || (((uintptr_t)x | (uintptr_t)codes) & 15) ||
-        (((uintptr_t)scales | (uintptr_t)out) & 1))
+        (((uintptr_t)scales | (uintptr_t)zeros) & 7) || ((uintptr_t)out & 1))
         return TERRACE_EINVAL;
     const int64_t busy = P < n_experts ? P : n_experts;      // experts that can hold a row
-    const int64_t mean = (P + busy - 1) / busy;
-    const int mt = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
-    const int R = 16 * mt;
-    const int64_t col_groups = swiglu ? (N / 2 + 15) / 16 : (N + 31) / 32;
-    const int64_t row_tiles = busy + (P - busy) / R + 1;     // the most there can be, and one for rows without expert
-    if (col_groups * row_tiles >= (int64_t)1 << 23) return TERRACE_EINVAL;   // 512 threads each: HIP's grid limit
-    int waves = 4;
-    if (mt == 1 && col_groups * (row_tiles - 1) * waves < 4096 && sh.blocks() > waves) waves = 8;
+    const int64_t out_cols = swiglu ? N / 2 : N;
+    // HIP's grid limit: 2^32 threads, 512 in a workgroup, each at least 16 columns of 16 rows
+    if ((out_cols + 15) / 16 * (busy + (P - busy) / 16 + 1) >= (int64_t)1 << 23) return TERRACE_EINVAL;
     const W4Args a{x, counts, (int)P, sh, (const u32x4 *)codes, (const uint16_t *)scales, (const uint8_t *)zeros, swiglu,
-                   (int)col_groups, out};
-    const unsigned grid = (unsigned)(col_groups * row_tiles);
-#define TERRACE_W4(DT)                                  \
-    if (mt == 1) launch_w4_g<DT, 1>(a, grid, waves, s); \
-    else if (mt == 2) launch_w4_g<DT, 2>(a, grid, waves, s); \
-    else launch_w4_g<DT, 4>(a, grid, waves, s)
+                   out, (int)out_cols, (int)sh.tiles(), (int)sh.blocks(), (int)(K / kBlockK), (int)(K % kBlockK / 32), 1, 1,
+                   1, 1};
+#define TERRACE_W4(DT)                              \
+    if (zeros) launch_w4<DT, true>(a, busy, s);     \
+    else launch_w4<DT, false>(a, busy, s)
     if (dtype == TERRACE_BF16) { TERRACE_W4(TERRACE_BF16); }
     else { TERRACE_W4(TERRACE_F16); }
 #undef TERRACE_W4

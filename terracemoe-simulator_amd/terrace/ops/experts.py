@@ -17,6 +17,7 @@ from .. import _hip
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _MAX_EXPERTS = 2048
+_MAX_WIDTH = 16384
 
 
 def _ops():
@@ -344,8 +345,7 @@ def block_norm(y, residual, post_weight=None, gate=None, pre_weight=None, *, sca
     and ``rms(v) = sqrt(mean(v^2) + eps)``.  ``y`` and ``residual`` are [..., H] of one shape, float32, bfloat16 or float16;
     the residual may be float32 beside a 16-bit ``y``.  ``h`` has the residual's dtype, ``n`` has ``y``'s; all arithmetic is
     fp32 and each output is rounded once (``n`` comes from the unrounded ``h``).  ``y`` None is the entry of the first
-    block: ``h`` is ``residual`` itself and ``n`` its norm.  Carries gradients to all five tensors.  H is at most 16384
-    where it is a multiple of 8, and at most 8192 otherwise."""
+    block: ``h`` is ``residual`` itself and ``n`` its norm.  Carries gradients to all five tensors.  H is at most 16384."""
     dev = _ready(y, residual, post_weight, gate, pre_weight)
     shape = residual.shape
     if residual.dim() < 1 or (y is not None and y.shape != shape):
@@ -357,8 +357,8 @@ def block_norm(y, residual, post_weight=None, gate=None, pre_weight=None, *, sca
     if any(t is not None and t.dtype not in _FLOATS for t in (y, residual, post_weight, gate, pre_weight)) or \
             (y is not None and residual.dtype not in (y.dtype, torch.float32)):
         raise RuntimeError("block_norm: float32, bfloat16 or float16; the residual of y's dtype or float32")
-    if not 0 < H <= 16384 or (H > 8192 and H % 8):
-        raise RuntimeError(f"block_norm: rows of {H}: up to 16384 where a multiple of 8, up to 8192 otherwise")
+    if not 0 < H <= _MAX_WIDTH:
+        raise RuntimeError(f"block_norm: rows of {H} elements; 1 to {_MAX_WIDTH} are taken")
     for name, v in (("post_weight", post_weight), ("pre_weight", pre_weight)):
         if v is not None and tuple(v.shape) != (H,):
             raise RuntimeError(f"block_norm: {name} must be [{H}], got {tuple(v.shape)}")

@@ -270,6 +270,8 @@ def check_w4(E, N, K, group, dtype, zeros, swiglu, counts, tail=0, seed=0):
     (4, 64, 256, 128, False, True, [1, 0, 0, 17]), (2, 50, 192, 64, True, True, [16, 15]), (5, 40, 320, 64, False, False, [0] * 5),
     (4, 48, 512, 128, True, False, [40, 33, 1, 0]), (2, 34, 288, 32, False, True, [70, 129]), (70, 18, 64, 64, False, False, [1, 0] * 35),
     (1, 256, 1024, 128, False, False, [1]), (3, 80, 160, 32, True, False, [64, 65, 63]),
+    (2, 11000, 160, 32, True, True, [130, 40]), (3, 20000, 128, 128, False, False, [20, 33, 1]), (1, 16400, 96, 32, False, True, [250]),
+    (2, 24010, 448, 64, True, False, [64, 64]), (1, 66000, 32, 32, False, False, [33]),
 ])
 def test_w4_products(E, N, K, group, zeros, swiglu, counts, dtype):
     check_w4(E, N, K, group, dtype, zeros, swiglu, counts, 0, E + N)
@@ -429,7 +431,8 @@ def tops_again(y, r, wp, gt, wn, scale, eps, dh, dn):
     (203, 1001, "f16", "f32", True, True, "token", True), (130, 264, "bf16", "bf16", True, False, "channel", True),
     (77, 4096, "f16", "f16", True, True, "channel", False), (300, 512, "f32", "f32", True, False, None, False),
     (33, 8192, "bf16", "bf16", True, True, "token", True), (9, 16384, "bf16", "f32", True, True, "channel", True),
-    (300, 9000, "f32", "f32", True, True, "token", True), (12, 8191, "bf16", "bf16", True, True, "channel", True),
+    (300, 9000, "f32", "f32", True, True, "token", True), (270, 8193, "bf16", "bf16", True, True, "channel", True), (5, 16383, "f16", "f32", True, True, "token", True),
+    (9, 15, "bf16", "bf16", True, True, "channel", True), (700, 7, "f16", "f16", True, True, "token", True), (12, 8191, "bf16", "bf16", True, True, "channel", True),
     (600, 72, "f16", "f16", True, True, "token", False), (40, 640, "bf16", "bf16", False, False, None, True),
     (21, 333, "f32", "f32", False, False, None, True), (1500, 1024, "f32", "f32", True, True, "channel", True),
 ])
@@ -540,7 +543,7 @@ def test_refusals():
                        ((y[:, :0], y[:, :0]), "rows of 0")]:
         with pytest.raises(RuntimeError, match=what):
             tops.block_norm(*args)
-    for H in (16392, 8193):
+    for H in (16385, 16392):
         big = torch.zeros((1, H), device=DEV)
         with pytest.raises(RuntimeError, match="rows of"):
             tops.block_norm(big, big)
