@@ -519,13 +519,13 @@ TERRACE_API int terrace_expert_unsort_grad(const void *rows, int row_dtype, cons
                                            int64_t hidden, int64_t n_rows, const int64_t *n_live, void *d_rows,
                                            void *d_weights, terrace_stream_t stream);
 
-/* 4-bit expert weights.  codes [n_experts,N,K/2] bytes (k even in the low nibble), scales [n_experts,N,K/group] 16-bit
- * floats, zeros [n_experts,N,K/group] bytes 0..15 or NULL (8 everywhere): weight = scale * (code - zero).  group is 32, 64
+/* 4-bit expert weights.  codes [n_experts,N,K/2] bytes (k even in the low nibble), scales [n_experts,N,K/group] of dtype
+ * (BF16 or F16), zeros [n_experts,N,K/group] bytes 0..15 or NULL (8 everywhere): weight = scale * (code - zero).  group is 32, 64
  * or 128 and divides K.  terrace_w4_pack lays them out for terrace_w4_linear, once per weight; terrace_w4_packed_bytes
  * tells the size of each packed plane (what: 0 codes, 1 scales, 2 zeros; 0 bytes: a shape that is not taken). */
 TERRACE_API size_t terrace_w4_packed_bytes(int n_experts, int64_t N, int64_t K, int group, int what);
-TERRACE_API int terrace_w4_pack(const void *codes, const void *scales, const void *zeros, int n_experts, int64_t N,
-                                int64_t K, int group, void *packed_codes, void *packed_scales, void *packed_zeros,
+TERRACE_API int terrace_w4_pack(const void *codes, const void *scales, const void *zeros, int dtype, int n_experts,
+                                int64_t N, int64_t K, int group, void *packed_codes, void *packed_scales, void *packed_zeros,
                                 terrace_stream_t stream);
 
 /* out[i] = W[e] x[i] for the rows i of expert e: x [P,K] and out [P,N] of dtype (BF16 or F16, the scales' type too),

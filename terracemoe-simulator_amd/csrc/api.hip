@@ -107,8 +107,8 @@ int run_expert_unsort_grad(const void *src, int src_dtype, const void *dy, int d
                            const void *weights, int w_dtype, int64_t T, int k, int64_t hidden, int64_t n_rows,
                            const int64_t *live, void *d_rows, void *d_weights, hipStream_t s);
 size_t w4_packed_bytes(int n_experts, int64_t N, int64_t K, int group, int what);
-int run_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int n_experts, int64_t N, int64_t K,
-                int group, void *packed_codes, void *packed_scales, void *packed_zeros, hipStream_t s);
+int run_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int dtype, int n_experts, int64_t N,
+                int64_t K, int group, void *packed_codes, void *packed_scales, void *packed_zeros, hipStream_t s);
 int run_w4_linear(const void *x, int dtype, int64_t P, const int64_t *counts, const void *codes, const void *scales,
                   const void *zeros, int n_experts, int64_t N, int64_t K, int group, int swiglu, void *out,
                   hipStream_t s);
@@ -575,9 +575,9 @@ size_t terrace_w4_packed_bytes(int n_experts, int64_t N, int64_t K, int group, i
     return what < 0 || what > 2 ? 0 : w4_packed_bytes(n_experts, N, K, group, what);
 }
 
-int terrace_w4_pack(const void *codes, const void *scales, const void *zeros, int n_experts, int64_t N, int64_t K,
+int terrace_w4_pack(const void *codes, const void *scales, const void *zeros, int dtype, int n_experts, int64_t N, int64_t K,
                     int group, void *packed_codes, void *packed_scales, void *packed_zeros, terrace_stream_t stream) {
-    return run_w4_pack((const uint8_t *)codes, scales, (const uint8_t *)zeros, n_experts, N, K, group, packed_codes,
+    return run_w4_pack((const uint8_t *)codes, scales, (const uint8_t *)zeros, dtype, n_experts, N, K, group, packed_codes,
                        packed_scales, packed_zeros, (hipStream_t)stream);
 }
 

@@ -16,13 +16,60 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------------------------
+// codes as 16-bit floats
+// ---------------------------------------------------------------------------------------------
+// A code c becomes the 16-bit float 16 + c by placing its four bits at the top of the mantissa of 16.0 (bf16: bits 3-6,
+// f16: bits 6-9): one turn and one and-or for two codes.  The constant is taken out again group by group,
+//   sum_k (c - z) x = sum_k (16 + c) x - (16 + z) * sum_k x,
+// the second sum by matrix instructions too (w4_use).  Everything is added in fp32, so the constant costs 2-3 bits of
+// 24, not of the inputs' 8 or 11.
+template <int DT>
+struct W4Type;
+template <>
+struct W4Type<TERRACE_BF16> {
+    typedef bf16x8 Frag;
+    static constexpr int kShift = 3;
+    static constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u, kOnes = 0x3F803F80u, kLess24 = 0xC1C0C1C0u;
+    static __device__ __forceinline__ f32x4 mfma(Frag a, Frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct W4Type<TERRACE_F16> {
+    typedef f16x8 Frag;
+    static constexpr int kShift = 6;
+    static constexpr uint32_t kMask = 0x03C003C0u, kBase = 0x4C004C00u, kOnes = 0x3C003C00u, kLess24 = 0xCE00CE00u;
+    static __device__ __forceinline__ f32x4 mfma(Frag a, Frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ typename W4Type<DT>::Frag w4_frag(uint32_t pair) {
+    const u32x4 v = {pair, pair, pair, pair};
+    return __builtin_bit_cast(typename W4Type<DT>::Frag, v);
+}
+// `base`: W4Type::kBase in a vector register (one and-or takes only one constant from elsewhere)
+template <int DT>
+__device__ __forceinline__ typename W4Type<DT>::Frag w4_expand(uint32_t w, uint32_t base) {
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = i == 0 ? w : __builtin_amdgcn_alignbit(w, w, 4 * i);
+        v[i] = (t & W4Type<DT>::kMask) | base;
+    }
+    return __builtin_bit_cast(typename W4Type<DT>::Frag, v);
+}
+
+// ---------------------------------------------------------------------------------------------
 // packed layout
 // ---------------------------------------------------------------------------------------------
 // Codes: [experts][column tiles of 16][blocks of 128 k][64 lanes][4 dwords].  Lane l holds column l % 16 of its tile and,
 // in dword s, the eight codes of k = 128 * block + 32 * s + 8 * (l / 16) + 0..7: what one 16x16x32 matrix instruction
 // takes from that lane, so a wave's load of a block is one contiguous kilobyte and any group of 32, 64 or 128 ends
-// with an instruction.  Inside a dword code 2i sits in nibble i and code 2i + 1 in nibble i + 4, 16 bits apart, so that one
-// shift and one mask leave a pair of neighbouring codes in the two halves of a register.  Scales and zero points:
+// with an instruction.  Inside a dword code 2i sits in nibble i and code 2i + 1 in nibble i + 4, 16 bits apart, and the
+// whole is turned left by the place a code takes in its 16-bit float (below): turning right by 4i puts a pair of
+// neighbouring codes where the two halves of a register want them.  Scales and zero points:
 // [experts][column tiles][blocks][16 columns][groups of a block], so a lane has those of a block in one load.  Columns
 // past N and k past K hold zeros.
 constexpr int kTileN = 16, kBlockK = 128;
@@ -42,7 +89,7 @@ struct W4Shape {
 };
 
 __global__ __launch_bounds__(kBlock) void w4_pack_codes_kernel(const uint8_t *__restrict__ codes, W4Shape sh,
-                                                               uint32_t *__restrict__ packed, int64_t total) {
+                                                               int turn, uint32_t *__restrict__ packed, int64_t total) {
     const int64_t step = (int64_t)gridDim.x * kBlock;
     for (int64_t d = (int64_t)blockIdx.x * kBlock + threadIdx.x; d < total; d += step) {
         const int s = (int)(d & 3), lane = (int)((d >> 2) & 63);
@@ -61,7 +108,7 @@ __global__ __launch_bounds__(kBlock) void w4_pack_codes_kernel(const uint8_t *__
                 out |= (b >> 4) << (4 * i + 16);
             }
         }
-        packed[d] = out;
+        packed[d] = out << turn | out >> (32 - turn);
     }
 }
 
@@ -89,10 +136,10 @@ size_t w4_packed_bytes(int n_experts, int64_t N, int64_t K, int group, int what)
     return cols * sh.groups() * (what == 1 ? 2 : 1);
 }
 
-int run_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int n_experts, int64_t N, int64_t K,
-                int group, void *packed_codes, void *packed_scales, void *packed_zeros, hipStream_t s) {
+int run_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int dtype, int n_experts, int64_t N,
+                int64_t K, int group, void *packed_codes, void *packed_scales, void *packed_zeros, hipStream_t s) {
     const W4Shape sh{n_experts, N, K, group};
-    if (!sh.ok() || !codes || !scales || !packed_codes || !packed_scales || (zeros != nullptr) != (packed_zeros != nullptr) ||
+    if (!sh.ok() || (dtype != TERRACE_BF16 && dtype != TERRACE_F16) || !codes || !scales || !packed_codes || !packed_scales || (zeros != nullptr) != (packed_zeros != nullptr) ||
         ((uintptr_t)packed_codes & 15) || (((uintptr_t)scales | (uintptr_t)packed_scales) & 1))
         return TERRACE_EINVAL;
     auto grid = [](int64_t n) {
@@ -101,7 +148,9 @@ int run_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, 
     };
     const int64_t dwords = (int64_t)(w4_packed_bytes(n_experts, N, K, group, 0) / 4);
     const int64_t groups = (int64_t)w4_packed_bytes(n_experts, N, K, group, 2);
-    w4_pack_codes_kernel<<<grid(dwords), kBlock, 0, s>>>(codes, sh, (uint32_t *)packed_codes, dwords);
+    w4_pack_codes_kernel<<<grid(dwords), kBlock, 0, s>>>(
+        codes, sh, dtype == TERRACE_BF16 ? W4Type<TERRACE_BF16>::kShift : W4Type<TERRACE_F16>::kShift,
+        (uint32_t *)packed_codes, dwords);
     w4_pack_groups_kernel<uint16_t><<<grid(groups), kBlock, 0, s>>>((const uint16_t *)scales, sh, (uint16_t *)packed_scales,
                                                                     groups);
     if (zeros)
@@ -112,44 +161,6 @@ int run_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, 
 // ---------------------------------------------------------------------------------------------
 // product
 // ---------------------------------------------------------------------------------------------
-// A code c becomes the 16-bit float 16 + c by placing its four bits at the top of the mantissa of 16.0 (bf16: bits 3-6,
-// f16: bits 6-9): two integer instructions for two codes.  The constant is taken out again after each group:
-//   sum_k (c - z) x = sum_k (16 + c) x - (16 + z) * sum_k x,
-// where sum_k x comes from one more matrix instruction per step against a column of ones, shared by all column tiles
-// of the wave.  Both sums are fp32, so the constant costs 2-3 bits of 24, not of the inputs' 8 or 11.
-template <int DT>
-struct W4Type;
-template <>
-struct W4Type<TERRACE_BF16> {
-    typedef bf16x8 Frag;
-    static constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u, kOnes = 0x3F803F80u;
-    static __device__ __forceinline__ uint32_t place(uint32_t w, int i) {
-        return i == 0 ? w << 3 : w >> (4 * i - 3);
-    }
-    static __device__ __forceinline__ f32x4 mfma(Frag a, Frag b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-};
-template <>
-struct W4Type<TERRACE_F16> {
-    typedef f16x8 Frag;
-    static constexpr uint32_t kMask = 0x03C003C0u, kBase = 0x4C004C00u, kOnes = 0x3C003C00u;
-    static __device__ __forceinline__ uint32_t place(uint32_t w, int i) {
-        return i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6);
-    }
-    static __device__ __forceinline__ f32x4 mfma(Frag a, Frag b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    }
-};
-
-template <int DT>
-__device__ __forceinline__ typename W4Type<DT>::Frag w4_expand(uint32_t w) {
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (W4Type<DT>::place(w, i) & W4Type<DT>::kMask) | W4Type<DT>::kBase;
-    return __builtin_bit_cast(typename W4Type<DT>::Frag, v);
-}
-
 // Which expert's rows a row tile holds.  Tiles of R rows are counted expert by expert; every wave finds its own by scans
 // over the counts, a lane an expert, 64 at a time.  Counts are the caller's device data: each is taken into [0, P] and the
 // sums saturate at P, so no count names a row outside the P rows.
@@ -261,73 +272,104 @@ struct W4Block {
     u32x4 w[T];
     static constexpr int kWords = GPB == 4 ? 2 : 1;
     uint32_t s[T][kWords];                                   // a scale in each half
-    uint32_t z[T];                                           // a zero point in each byte
+    uint32_t z[ZEROS ? T : 1];                               // a zero point in each byte
+    template <bool STREAM>
     __device__ __forceinline__ void fetch(const W4Expert &e, const W4Column *col, int b) {
         const uint8_t *codes = e.codes + (int64_t)b * 1024, *scales = e.scales + (int64_t)b * (2 * GPB * kTileN);
+        const uint8_t *zeros = ZEROS ? e.zeros + (int64_t)b * (GPB * kTileN) : nullptr;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            w[t] = *(const u32x4 *)(codes + col[t].codes);
-            const auto v = *(const typename GroupBits<GPB>::S *)(scales + 2u * col[t].groups);
-            if constexpr (GPB == 4) s[t][0] = v[0], s[t][1] = v[1];
-            else s[t][0] = v;
-        }
-        if constexpr (ZEROS) {
-            const uint8_t *zeros = e.zeros + (int64_t)b * (GPB * kTileN);
-#pragma unroll
-            for (int t = 0; t < T; ++t) z[t] = *(const typename GroupBits<GPB>::Z *)(zeros + col[t].groups);
-        } else {
-#pragma unroll
-            for (int t = 0; t < T; ++t) z[t] = 0x08080808u;
+            // a scalar base and a 32-bit offset: the offsets are kept apart, or the compiler adds them up ahead of the
+            // loop and pays a 64-bit vector add a load
+            uint32_t at = col[t].codes, group = col[t].groups;
+            asm volatile("" : "+v"(at), "+v"(group));
+            w[t] = STREAM ? ld_stream((const u32x4 *)(codes + at)) : *(const u32x4 *)(codes + at);
+            const auto v = *(const typename GroupBits<GPB>::S *)(scales + 2u * group);
+            if constexpr (GPB == 4) {
+                s[t][0] = v[0];
+                s[t][1] = v[1];
+            } else {
+                s[t][0] = v;
+            }
+            if constexpr (ZEROS) z[t] = *(const typename GroupBits<GPB>::Z *)(zeros + group);
         }
     }
 };
 
-// total += the block's products: x(m, s) gives the rows' fragment of step s.
+// total += the block's products: x(m, s) gives the rows' fragment of step s.  What takes the constant out:
+//   no zero points       sum_k -24 x, summed first by matrix instructions, is where every tile's sum of a group starts
+//   ZEROS, one row tile  a matrix instruction more per tile and step, against -(16 + z)
+//   ZEROS, more          sum_k x by matrix instructions, once for all tiles, and a multiply-add per result
 template <int DT, int MT, int T, int GS, bool ZEROS, typename X>
 __device__ __forceinline__ void w4_use(W4Block<T, 4 / GS, ZEROS> &k, X x, f32x4 (*total)[T]) {
-    typedef typename W4Type<DT>::Frag Frag;
-    const u32x4 ones4 = {W4Type<DT>::kOnes, W4Type<DT>::kOnes, W4Type<DT>::kOnes, W4Type<DT>::kOnes};
-    const Frag ones = __builtin_bit_cast(Frag, ones4);
+    typedef W4Type<DT> Type;
+    typedef typename Type::Frag Frag;
+    uint32_t base = Type::kBase;
+    asm volatile("" : "+v"(base));
     // what was fetched stays as it came until here: without this the compiler unpacks it where it arrives, and a ring of
     // unpacked blocks does not fit the registers
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-        asm volatile("" : "+v"(k.w[t]), "+v"(k.z[t]));
+        asm volatile("" : "+v"(k.w[t]));
+        if constexpr (ZEROS) asm volatile("" : "+v"(k.z[t]));
 #pragma unroll
         for (int i = 0; i < W4Block<T, 4 / GS, ZEROS>::kWords; ++i) asm volatile("" : "+v"(k.s[t][i]));
     }
-    f32x4 acc[MT][T], sum[MT];
+    constexpr bool kSum = ZEROS && MT > 1, kTile = ZEROS && MT == 1;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+    for (int g = 0; g < 4 / GS; ++g) {
+        f32x4 acc[MT][T], sum[MT];
         const f32x4 zero = {0, 0, 0, 0};
-        const bool first = s % GS == 0;
-        Frag xs[MT];
+        if constexpr (!kTile) {
+            const Frag c = w4_frag<DT>(kSum ? Type::kOnes : Type::kLess24);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            xs[m] = __builtin_bit_cast(Frag, x(m, s));
-            sum[m] = W4Type<DT>::mfma(xs[m], ones, first ? zero : sum[m]);
+            for (int m = 0; m < MT; ++m) {
+                sum[m] = zero;
+#pragma unroll
+                for (int s = 0; s < GS; ++s) sum[m] = Type::mfma(__builtin_bit_cast(Frag, x(m, g * GS + s)), c, sum[m]);
+            }
+        }
+        Frag less[T];
+        if constexpr (kTile) {
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const uint32_t z = (k.z[t] >> (8 * g)) & 0xFFu, half = 0x8000u | (Type::kBase & 0x7FFFu) | (z << Type::kShift);
+                less[t] = w4_frag<DT>(half | half << 16);
+            }
         }
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const Frag f = w4_expand<DT>(k.w[t][s]);
+        for (int s = 0; s < GS; ++s) {
+            Frag xs[MT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][t] = W4Type<DT>::mfma(xs[m], f, first ? zero : acc[m][t]);
+            for (int m = 0; m < MT; ++m) xs[m] = __builtin_bit_cast(Frag, x(m, g * GS + s));
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const Frag f = w4_expand<DT>(k.w[t][g * GS + s], base);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const f32x4 from = s ? acc[m][t] : ZEROS ? zero : sum[m];
+                    acc[m][t] = Type::mfma(xs[m], f, from);
+                    if constexpr (kTile) acc[m][t] = Type::mfma(xs[m], less[t], acc[m][t]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);               // one step's expanded codes at a time in registers
         }
-        __builtin_amdgcn_sched_barrier(0);                   // one step's expanded codes at a time in registers
-        if (s % GS != GS - 1) continue;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             float scale;
-            const int g = s / GS;
-            const uint32_t bits = g & 1 ? k.s[t][g / 2] >> 16 : k.s[t][g / 2] & 0xFFFFu;
-            if constexpr (DT == TERRACE_BF16) scale = bf16_bits_to_f32(bits);
-            else scale = __half2float(__ushort_as_half((unsigned short)bits));
-            const float off = -16.0f - (float)((k.z[t] >> (8 * g)) & 0xFFu);
+            const uint32_t word = k.s[t][g / 2];
+            if constexpr (DT == TERRACE_BF16) scale = g & 1 ? __uint_as_float(word & 0xFFFF0000u) : __uint_as_float(word << 16);
+            else scale = __half2float(__ushort_as_half((unsigned short)(g & 1 ? word >> 16 : word)));
+            float off = 0.0f;
+            if constexpr (kSum) off = -16.0f - (float)((k.z[t] >> (8 * g)) & 0xFFu);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    total[m][t][i] = __fmaf_rn(scale, __fmaf_rn(off, sum[m][i], acc[m][t][i]), total[m][t][i]);
+                for (int i = 0; i < 4; ++i) {
+                    float v = acc[m][t][i];
+                    if constexpr (kSum) v = __fmaf_rn(off, sum[m][i], v);
+                    total[m][t][i] = __fmaf_rn(scale, v, total[m][t][i]);
+                }
         }
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -339,11 +381,11 @@ __device__ __forceinline__ float w4_swiglu(float gate, float up) { return gate /
 // is the work of `split` waves that share out the blocks of k and are joined in LDS, in order; a workgroup holds 4 or 8
 // waves and so 4 / split or 8 / split sets.  The rows' fragments come straight from memory (a few rows: L1 and L2), and
 // codes and rows are fetched kAhead blocks ahead, because the codes come from HBM and nothing else hides their latency.
-constexpr int kAhead = 3;
+constexpr int kAhead = 2;
 constexpr int kMaxSplit = 8;
 
 template <int DT, int GS, bool ZEROS>
-__global__ __launch_bounds__(kMaxSplit * kWave) __attribute__((amdgpu_waves_per_eu(4))) void w4_few_kernel(W4Args a) {
+__global__ __launch_bounds__(kMaxSplit * kWave) void w4_few_kernel(W4Args a) {
     __shared__ float lds[kMaxSplit][8][kWave];
     const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_in_block());
     const int cb = (int)(blockIdx.x % (unsigned)a.col_blocks), tile = (int)(blockIdx.x / (unsigned)a.col_blocks);
@@ -367,10 +409,12 @@ __global__ __launch_bounds__(kMaxSplit * kWave) __attribute__((amdgpu_waves_per_
         u32x4 x[4];
     };
     auto fetch = [&](int b, Block &f) {
-        f.k.fetch(we, col, b);
+        f.k.template fetch<true>(we, col, b);
         const uint8_t *xb = xt + (int64_t)b * (2 * kBlockK);
+        uint32_t o = xo;
+        asm volatile("" : "+v"(o));
 #pragma unroll
-        for (int s = 0; s < 4; ++s) f.x[s] = *(const u32x4 *)(xb + xo + 64 * s);
+        for (int s = 0; s < 4; ++s) f.x[s] = *(const u32x4 *)(xb + o + 64 * s);
     };
     auto use = [&](Block &f) {
         w4_use<DT, 1, 2, GS, ZEROS>(f.k, [&](int, int s) { return f.x[s]; }, total);
@@ -379,17 +423,22 @@ __global__ __launch_bounds__(kMaxSplit * kWave) __attribute__((amdgpu_waves_per_
         Block ring[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) fetch(b0 + i < b1 ? b0 + i : b1 - 1, ring[i]);
-        for (int b = b0; b < b1; b += kAhead) {              // past the end the last block is fetched again, from cache
+        int b = b0;
+        for (; b + kAhead <= b1; b += kAhead) {              // past the end the last block is fetched again, from cache
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                if (b + i < b1) use(ring[i]);
+                use(ring[i]);
                 fetch(b + kAhead + i < b1 ? b + kAhead + i : b1 - 1, ring[i]);
             }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) {
+            if (b + i < b1) use(ring[i]);
         }
     }
     if (a.rest && part == a.split - 1) {                     // a K that is no multiple of 128: zeros past it
         Block f;
-        f.k.fetch(we, col, a.full);
+        f.k.template fetch<true>(we, col, a.full);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             f.x[s] = zero_of<u32x4>();
@@ -432,13 +481,16 @@ __global__ __launch_bounds__(kMaxSplit * kWave) __attribute__((amdgpu_waves_per_
 // Tens of rows: tiles of 16 * MT.  A workgroup of four waves makes 256 columns, each wave four tiles (with `swiglu` two of
 // each half), so the rows of a block of k are read once for 256 columns: they go through LDS in the order the matrix
 // instructions take them, one block ahead, while every wave streams its own codes two blocks ahead.
+constexpr int kManyTiles = 4;
+// (two waves a SIMD at least: with a whole SIMD's registers to itself the compiler puts the sums into accumulation
+// registers and copies each out again before the multiply-add, a fifth of the kernel's instructions)
 template <int DT, int MT, int GS, bool ZEROS>
-__global__ __launch_bounds__(4 * kWave) void w4_many_kernel(W4Args a) {
-    constexpr int R = 16 * MT, T = 4;
+__global__ __launch_bounds__(4 * kWave, 2) void w4_many_kernel(W4Args a) {
+    constexpr int R = 16 * MT, T = kManyTiles;
     __shared__ u32x4 rows[2][4][MT][kWave];                  // [buffer][step][16 rows][lane]
     const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_in_block());
     const int cb = (int)(blockIdx.x % (unsigned)a.col_blocks), tile = (int)(blockIdx.x / (unsigned)a.col_blocks);
-    const int width = a.swiglu ? 32 : 64, lo = cb * 4 * width;
+    const int width = a.swiglu ? T * 8 : T * 16, lo = cb * 4 * width;
     const RowTile rt = find_tile(a.counts, a.sh.n_experts, a.P, R, tile);
     if (rt.expert < 0) {
         w4_zero_rows(a, rt, tile, lo, lo + 4 * width);
@@ -453,26 +505,32 @@ __global__ __launch_bounds__(4 * kWave) void w4_many_kernel(W4Args a) {
         at[t] = lo + w * width + c16 + (a.swiglu ? (t >> 1) * 16 + (t & 1) * a.out_cols : t * 16);
         col[t] = w4_column(a, at[t], q, 4 / GS);
     }
-    // wave w brings step w of a block: rows past the tile's last repeat it (their results are dropped)
+    // wave w brings step w of a block: rows past the tile's last repeat it (their results are dropped), and a step past K
+    // reads what is there and is masked to zeros, so that every load of the loop is unconditional
+    const bool short_k = a.full == 0 && w >= a.rest;
     const uint8_t *xt = (const uint8_t *)a.x + (int64_t)rt.first * a.sh.K * 2;
     uint32_t xo[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int r = 16 * m + c16 < rt.rows ? 16 * m + c16 : rt.rows - 1;
-        xo[m] = (uint32_t)(r * (int)a.sh.K + 32 * w + 8 * q) * 2u;
+        xo[m] = (uint32_t)(r * (int)a.sh.K + (short_k ? 0 : 32 * w) + 8 * q) * 2u;
     }
     const int blocks = a.blocks;
-    u32x4 xn[MT];
-    auto bring = [&](int b) {                                // the next block, or the last once more; zeros past K
+    u32x4 xn[2][MT];
+    auto bring = [&](int b, int i) {
         const int c = b < blocks ? b : blocks - 1;
-        const bool in = c < a.full || w < a.rest;
-        const uint8_t *xb = xt + (int64_t)(in ? c : 0) * (2 * kBlockK);
+        const uint8_t *xb = xt + (int64_t)(c < a.full || w < a.rest ? c : 0) * (2 * kBlockK);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) xn[m] = in ? *(const u32x4 *)(xb + xo[m]) : zero_of<u32x4>();
+        for (int m = 0; m < MT; ++m) {
+            uint32_t o = xo[m];
+            asm volatile("" : "+v"(o));
+            xn[i][m] = *(const u32x4 *)(xb + o);
+        }
     };
-    auto place = [&](int buf) {
+    auto place = [&](int b, int i) {
+        const uint32_t mask = b < a.full || w < a.rest ? 0xFFFFFFFFu : 0u;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) rows[buf][w][m][lane] = xn[m];
+        for (int m = 0; m < MT; ++m) rows[i][w][m][lane] = xn[i][m] & mask;
     };
     f32x4 total[MT][T];
 #pragma unroll
@@ -480,22 +538,27 @@ __global__ __launch_bounds__(4 * kWave) void w4_many_kernel(W4Args a) {
 #pragma unroll
         for (int t = 0; t < T; ++t) total[m][t] = f32x4{0, 0, 0, 0};
     W4Block<T, 4 / GS, ZEROS> ring[2];
-    ring[0].fetch(we, col, 0);
-    ring[1].fetch(we, col, blocks > 1 ? 1 : 0);
-    bring(0);
-    place(0);
+    auto use = [&](int i) {
+        w4_use<DT, MT, T, GS, ZEROS>(ring[i], [&](int m, int s) { return rows[i][s][m][lane]; }, total);
+    };
+    bring(0, 0);
+    ring[0].template fetch<false>(we, col, 0);
+    bring(1, 1);
+    ring[1].template fetch<false>(we, col, blocks > 1 ? 1 : 0);
+    place(0, 0);
     __syncthreads();
-    for (int b = 0; b < blocks; b += 2) {
+    int b = 0;
+    for (; b + 1 < blocks; b += 2) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            bring(b + i + 1);
-            if (b + i < blocks)
-                w4_use<DT, MT, T, GS, ZEROS>(ring[i], [&](int m, int s) { return rows[i][s][m][lane]; }, total);
-            ring[i].fetch(we, col, b + i + 2 < blocks ? b + i + 2 : blocks - 1);
-            place(1 - i);
+            bring(b + i + 2, i);
+            use(i);
+            ring[i].template fetch<false>(we, col, b + i + 2 < blocks ? b + i + 2 : blocks - 1);
+            place(b + i + 1, 1 - i);
             __syncthreads();
         }
     }
+    if (b < blocks) use(0);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -523,8 +586,8 @@ static void launch_w4(W4Args a, int64_t busy, hipStream_t s) {
     auto tiles = [&](int64_t R) { return busy + (P - busy) / R + 1; };
     const int64_t mean = (P + busy - 1) / busy;
     const int mt = mean <= 32 ? 2 : 4;
-    const int64_t wide = a.swiglu ? (a.out_cols + 127) / 128 : (a.out_cols + 255) / 256;
-    if (mean > 16 && wide * (tiles(16 * mt) - 1) >= 256) {
+    const int64_t per_wide = kManyTiles * (a.swiglu ? 32 : 64), wide = (a.out_cols + per_wide - 1) / per_wide;
+    if (mean > 8 && wide * (tiles(16 * mt) - 1) >= 256) {
         a.col_blocks = (int)wide;
         const unsigned grid = (unsigned)(wide * tiles(16 * mt));
 #define TERRACE_MANY(MT)                                                                            \

@@ -99,7 +99,7 @@ SIGNATURES = {
     "terrace_expert_sort": (_I, [_P, _P, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "terrace_expert_unsort_grad": (_I, [_P, _I, _P, _I, _P, _P, _I, _L, _I, _L, _L, _P, _P, _P, _P]),
     "terrace_w4_packed_bytes": (_Z, [_I, _L, _L, _I, _I]),
-    "terrace_w4_pack": (_I, [_P, _P, _P, _I, _L, _L, _I, _P, _P, _P, _P]),
+    "terrace_w4_pack": (_I, [_P, _P, _P, _I, _I, _L, _L, _I, _P, _P, _P, _P]),
     "terrace_w4_linear": (_I, [_P, _I, _L, _P, _P, _P, _P, _I, _L, _L, _I, _I, _P, _P]),
     "terrace_block_norm": (_I, [_P, _I, _P, _I, _P, _I, _P, _I, _I, _P, _I, _F, _F, _L, _L, _P, _P, _P, _P]),
     "terrace_block_norm_grad_workspace": (_Z, [_L, _L]),

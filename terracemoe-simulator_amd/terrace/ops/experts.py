@@ -241,8 +241,8 @@ def w4_pack(codes, scales, zeros=None) -> W4Weights:
     out_codes = torch.empty((sizes[0],), dtype=torch.uint8, device=dev)
     out_scales = torch.empty((sizes[1] // 2,), dtype=scales.dtype, device=dev)
     out_zeros = None if zeros is None else torch.empty((sizes[2],), dtype=torch.uint8, device=dev)
-    _call(dev, "terrace_w4_pack", codes.data_ptr(), scales.data_ptr(), _hip.ptr(zeros), E, N, K, group,
-          out_codes.data_ptr(), out_scales.data_ptr(), _hip.ptr(out_zeros), _hip.stream(dev))
+    _call(dev, "terrace_w4_pack", codes.data_ptr(), scales.data_ptr(), _hip.ptr(zeros), _hip.float_code(scales.dtype), E, N, K,
+          group, out_codes.data_ptr(), out_scales.data_ptr(), _hip.ptr(out_zeros), _hip.stream(dev))
     return W4Weights(out_codes, out_scales, out_zeros, E, N, K, group, scales.dtype)
 
 
