@@ -217,6 +217,11 @@ def stream(device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(index: int) -> int:
+    """The handle of the HIP stream torch currently launches on for device ``index``."""
+    return _RAW_STREAM(index) if _RAW_STREAM is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def row_arg(t) -> int:
     """The ``row_bytes`` argument for a 2-D row tensor: its width in bytes, or -- for a row-pitched view (unit
     stride inside a row, rows further apart than they are wide) -- TERRACE_ROW_PITCHED(width, pitch)."""

@@ -8,49 +8,57 @@ enqueues on the current stream of its tensors' device.
 """
 from __future__ import annotations
 
-from typing import NamedTuple
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _hip
+from .. import ops as _ops
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_CODE = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16, torch.float16: _hip.F16}
 _MAX_EXPERTS = 2048
 _MAX_WIDTH = 16384
+_CURRENT = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _ops():
-    from .. import ops           # deferred: the package imports this module
-    return ops
+def _ready(*tensors) -> int:
+    """The library is loaded and the tensors (None: absent) share one ROCm device, whose index is returned."""
+    _ops._require()
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _hip.need_device(t)
+        at = t.get_device()
+        if index < 0:
+            index = at
+        elif at != index:
+            raise RuntimeError(f"terrace: tensors on cuda:{index} and on cuda:{at} in one call")
+    return index
 
 
-def _ready(*tensors):
-    """The library is loaded and the tensors share one ROCm device, which is returned."""
-    _ops()._require()
-    _hip.need_device(*tensors)
-    given = [t for t in tensors if t is not None]
-    dev = given[0].device
-    for t in given[1:]:
-        if t.device != dev:
-            raise RuntimeError(f"terrace: tensors on {dev} and on {t.device} in one call")
-    return dev
-
-
-def _call(dev, name, *args):
-    """One library call with ``dev`` current: a kernel is launched from the device its stream belongs to."""
-    if dev.index == torch.cuda.current_device():
-        _hip.call(name, *args)
+def _enqueue(index: int, name: str, *args):
+    """One library call on the current stream of device ``index``, with that device current: a kernel is launched from
+    the device its stream belongs to."""
+    if index == _CURRENT():
+        _hip.call(name, *args, _hip.raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            _hip.call(name, *args)
+        with torch.cuda.device(index):
+            _hip.call(name, *args, _hip.raw_stream(index))
+
+
+def _at(t):
+    """Address of a tensor for an argument that may be absent."""
+    return None if t is None else t.data_ptr()
 
 
 def _movable_rows(t):
     """``t`` as the row movers take it: packed, or on a kilobyte pitch; else a packed copy."""
+    if t.is_contiguous():
+        return t
     pitch = t.stride(0) * t.element_size() if t.shape[0] > 1 else 0
-    if _hip.is_rows(t) and not t.is_contiguous() and pitch % 1024 == 0 and t.data_ptr() % 16 == 0 and \
-            (t.shape[1] * t.element_size()) % 16 == 0:
+    if _hip.is_rows(t) and pitch % 1024 == 0 and t.data_ptr() % 16 == 0 and (t.shape[1] * t.element_size()) % 16 == 0:
         return t
     return t.contiguous()
 
@@ -59,7 +67,8 @@ def _aligned(t):
     """``t`` packed and on a 16-byte boundary (a copy only when it is not)."""
     if t is None:
         return None
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -67,52 +76,85 @@ def _aligned(t):
 # tokens to expert order and back
 # --------------------------------------------------------------------------------------
 
-class ExpertPlan(NamedTuple):
-    """Where :func:`expert_sort` put each (token, expert) pair."""
-    where: torch.Tensor                 # [T, k] int64: its row in expert order, -1 for a pair without an expert
-    tokens_per_expert: torch.Tensor     # [n_experts] int64
-    offsets: torch.Tensor               # [n_experts + 1] int64: first row of each expert; the last entry counts all pairs
-    status: torch.Tensor                # the library's status words: FAULT_ID_RANGE when an id was >= n_experts
+class ExpertPlan:
+    """Where :func:`expert_sort` put each (token, expert) pair.  The planes share one allocation and become tensors of
+    their own when first read:
+
+    ``where``              [T, k] int64: the pair's row in expert order, -1 for a pair without an expert
+    ``tokens_per_expert``  [n_experts] int64
+    ``offsets``            [n_experts + 1] int64: first row of each expert; the last entry counts the pairs with one
+    ``status``             the library's status words: FAULT_ID_RANGE when an id was >= n_experts"""
+
+    __slots__ = ("planes", "T", "k", "n_experts", "_made")
+
+    def __init__(self, planes, T, k, n_experts):
+        self.planes, self.T, self.k, self.n_experts, self._made = planes, T, k, n_experts, {}
+
+    @staticmethod
+    def words(T, k, n_experts):
+        """int64 words of the planes: places, counts, offsets, status."""
+        return T * k + 2 * n_experts + 3
+
+    def _plane(self, name, lo, n):
+        t = self._made.get(name)
+        if t is None:
+            t = self._made[name] = self.planes[lo:lo + n]
+        return t
+
+    @property
+    def where(self):
+        return self._plane("where", 0, self.T * self.k).view(self.T, self.k)
+
+    @property
+    def tokens_per_expert(self):
+        return self._plane("tokens_per_expert", self.T * self.k, self.n_experts)
+
+    @property
+    def offsets(self):
+        return self._plane("offsets", self.T * self.k + self.n_experts, self.n_experts + 1)
+
+    @property
+    def status(self):
+        return self._plane("status", self.T * self.k + 2 * self.n_experts + 1, 2).view(torch.int32)
 
 
-def _sort_raw(x, expert_idx, n_experts):
-    dev = x.device
-    T, k = expert_idx.shape
+def _sort_raw(index, x, expert_idx, planes, T, k, n):
     x = _movable_rows(x)
     expert_idx = expert_idx.contiguous()
-    rows = _hip.empty_rows(T * k, x)
-    # the index planes share one allocation: [T*k] places, [n] counts, [n + 1] offsets, 2 words of status
-    n = n_experts
-    planes = torch.empty((T * k + 2 * n + 3,), dtype=torch.int64, device=dev)
-    where, counts, offsets, words = planes.split((T * k, n, n + 1, 2))
+    rows = torch.empty((T * k, x.shape[1]), dtype=x.dtype, device=x.device) if x.is_contiguous() else \
+        _hip.empty_rows(T * k, x)
     need = _hip.query("terrace_expert_sort_workspace", T, k, n)
-    ws = _hip.workspace(need, dev) if need > 256 else None
+    ws = _hip.workspace(need, x.device) if need > 256 else None      # 256: the one-launch form, which needs none
     base = planes.data_ptr()
-    _call(dev, "terrace_expert_sort", x.data_ptr(), expert_idx.data_ptr(), T, _hip.row_arg(x), k, n, rows.data_ptr(), base,
-          base + 8 * T * k, base + 8 * (T * k + n), base + 8 * (T * k + 2 * n + 1), _hip.ptr(ws),
-          0 if ws is None else ws.numel(), _hip.stream(dev))
-    return rows, where.view(T, k), counts, offsets, words.view(torch.int32)
+    counts = base + 8 * T * k
+    _enqueue(index, "terrace_expert_sort", x.data_ptr(), expert_idx.data_ptr(), T, _hip.row_arg(x), k, n, rows.data_ptr(),
+             base, counts, counts + 8 * n, counts + 8 * (2 * n + 1), _at(ws), need if ws is not None else 0)
+    return rows
+
+
+def _combine(index, rows, where_at, weights, T, k, out_dtype):
+    """The combine over the [T, k] places at address ``where_at``: rows packed, weights packed or None."""
+    out = torch.empty((T, rows.shape[1]), dtype=out_dtype, device=rows.device)
+    _enqueue(index, "terrace_combine", rows.data_ptr(), rows.shape[0], _CODE[rows.dtype], where_at, _at(weights),
+             0 if weights is None else _CODE[weights.dtype], T, k, rows.shape[1], out.data_ptr(), _CODE[out_dtype])
+    return out
 
 
 class _ExpertSortFn(torch.autograd.Function):
     """rows[where[t, j]] = x[t]; adjoint: a token sums the gradients of its k rows in column order."""
 
     @staticmethod
-    def forward(ctx, x, expert_idx, n_experts):
-        rows, where, counts, offsets, status = _sort_raw(x, expert_idx, n_experts)
-        ctx.save_for_backward(where)
-        ctx.mark_non_differentiable(where, counts, offsets, status)
-        ctx.set_materialize_grads(False)
-        ctx.dtype = x.dtype
-        return rows, where, counts, offsets, status
+    def forward(ctx, x, expert_idx, planes, T, k, n):
+        ctx.save_for_backward(planes)
+        ctx.geom = (T, k, x.dtype)
+        return _sort_raw(x.get_device(), x, expert_idx, planes, T, k, n)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, g, *_):
-        (where,) = ctx.saved_tensors
-        if g is None:
-            return None, None, None
-        return _ops().combine(g.contiguous(), where, None, out_dtype=ctx.dtype), None, None
+    def backward(ctx, g):
+        (planes,) = ctx.saved_tensors
+        T, k, dtype = ctx.geom
+        return _combine(g.get_device(), g.contiguous(), planes.data_ptr(), None, T, k, dtype), None, None, None, None, None
 
 
 def expert_sort(x, expert_idx, n_experts: int):
@@ -122,51 +164,51 @@ def expert_sort(x, expert_idx, n_experts: int):
     keep their order (token, then column).  An id below 0 is a pair without an expert here -- another rank's, or masked
     -- and one past ``n_experts`` is treated the same and reported in ``plan.status``; such a pair has ``where`` -1, and
     the rows behind the last live one are zeros.  A token may have no expert at all.  ``rows`` carries gradients to ``x``
-    (any dtype may be sorted; gradients need a float one).  ``plan.tokens_per_expert`` is what :func:`expert_linear_w4`
-    takes, ``plan.where`` what ``combine`` takes.  At most 2048 experts.  Up to 2048 pairs the call is one launch."""
-    _ready(x, expert_idx)
+    (any dtype may be sorted; gradients need float32, bfloat16 or float16).  ``plan.tokens_per_expert`` is what
+    :func:`expert_linear_w4` takes, ``plan.where`` what ``combine`` takes.  At most 2048 experts.  Up to 2048 pairs the
+    call is one launch."""
+    index = _ready(x, expert_idx)
     if x.dim() != 2 or expert_idx.dim() != 2 or x.shape[0] != expert_idx.shape[0]:
         raise RuntimeError(f"expert_sort: x {tuple(x.shape)} and expert_idx {tuple(expert_idx.shape)} must be [T, H] "
                            f"and [T, k]")
     if expert_idx.dtype != torch.int64:
         raise RuntimeError("expert_sort: expert_idx must be int64")
-    if not 0 < n_experts <= _MAX_EXPERTS or expert_idx.shape[1] < 1:
-        raise RuntimeError(f"expert_sort: 1 to {_MAX_EXPERTS} experts and at least one column, got {n_experts} and "
-                           f"{expert_idx.shape[1]}")
-    if torch.is_grad_enabled() and x.requires_grad:
-        rows, *plan = _ExpertSortFn.apply(x, expert_idx, int(n_experts))
+    T, k = expert_idx.shape
+    n = int(n_experts)
+    if not 0 < n <= _MAX_EXPERTS or k < 1:
+        raise RuntimeError(f"expert_sort: 1 to {_MAX_EXPERTS} experts and at least one column, got {n} and {k}")
+    planes = torch.empty((ExpertPlan.words(T, k, n),), dtype=torch.int64, device=x.device)
+    if x.requires_grad and torch.is_grad_enabled():
+        if x.dtype not in _FLOATS:
+            raise RuntimeError(f"expert_sort: gradients need float32, bfloat16 or float16 rows, got {x.dtype}")
+        rows = _ExpertSortFn.apply(x, expert_idx, planes, T, k, n)
     else:
-        rows, *plan = _sort_raw(x, expert_idx, int(n_experts))
-    return rows, ExpertPlan(*plan)
+        rows = _sort_raw(index, x, expert_idx, planes, T, k, n)
+    return rows, ExpertPlan(planes, T, k, n)
 
 
 class _ExpertUnsortFn(torch.autograd.Function):
     """y[t] = sum_j weights[t, j] * rows[where[t, j]]; adjoint: one pass over dy and the rows."""
 
     @staticmethod
-    def forward(ctx, rows, weights, where, offsets, out_dtype):
-        rows = rows.contiguous()
-        ctx.save_for_backward(rows, weights, where, offsets)
-        ctx.set_materialize_grads(False)
-        return _ops().combine(rows, where, weights, out_dtype=out_dtype)
+    def forward(ctx, rows, weights, planes, T, k, n, out_dtype):
+        ctx.save_for_backward(rows, weights, planes)
+        ctx.geom = (T, k, n)
+        return _combine(rows.get_device(), rows, planes.data_ptr(), weights, T, k, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        rows, weights, where, offsets = ctx.saved_tensors
-        if dy is None:
-            return (None,) * 5
+        rows, weights, planes = ctx.saved_tensors
+        T, k, n = ctx.geom
         dy = dy.contiguous()
-        T, k = where.shape
-        want_rows, want_w = ctx.needs_input_grad[0], weights is not None and ctx.needs_input_grad[1]
-        d_rows = torch.empty_like(rows) if want_rows else None
-        w = None if weights is None else weights.contiguous()
-        d_w = torch.empty_like(w) if want_w else None
-        _call(rows.device, "terrace_expert_unsort_grad", rows.data_ptr(), _hip.float_code(rows.dtype), dy.data_ptr(),
-              _hip.float_code(dy.dtype), where.data_ptr(), _hip.ptr(w), 0 if w is None else _hip.float_code(w.dtype), T, k,
-              rows.shape[1], rows.shape[0], offsets.data_ptr() + 8 * (offsets.numel() - 1), _hip.ptr(d_rows),
-              _hip.ptr(d_w), _hip.stream(rows.device))
-        return d_rows, d_w, None, None, None
+        d_rows = torch.empty_like(rows) if ctx.needs_input_grad[0] else None
+        d_w = torch.empty_like(weights) if weights is not None and ctx.needs_input_grad[1] else None
+        where = planes.data_ptr()
+        _enqueue(rows.get_device(), "terrace_expert_unsort_grad", rows.data_ptr(), _CODE[rows.dtype], dy.data_ptr(),
+                 _CODE[dy.dtype], where, _at(weights), 0 if weights is None else _CODE[weights.dtype], T, k, rows.shape[1],
+                 rows.shape[0], where + 8 * (T * k + 2 * n), _at(d_rows), _at(d_w))
+        return d_rows, d_w, None, None, None, None, None
 
 
 def expert_unsort(rows, weights, plan: ExpertPlan, out_dtype=None):
@@ -177,22 +219,20 @@ def expert_unsort(rows, weights, plan: ExpertPlan, out_dtype=None):
     ``weights`` [T, k] of any of these types, or None for plain sums.  A pair without an expert contributes nothing and
     a token without any is a zero row, whatever ``rows`` holds behind the live rows.  Carries gradients to ``rows``
     (zeros behind the live rows) and ``weights`` (0 where there is no expert)."""
-    dev = _ready(rows, weights, plan.where, plan.offsets)
-    where = plan.where
-    if rows.dim() != 2 or rows.shape[0] != where.numel():
-        raise RuntimeError(f"expert_unsort: rows {tuple(rows.shape)} does not have one row per pair of the plan "
-                           f"({where.numel()})")
-    if rows.dtype not in _FLOATS or (weights is not None and weights.dtype not in _FLOATS) or \
-            (out_dtype or rows.dtype) not in _FLOATS:
+    index = _ready(rows, weights, plan.planes)
+    T, k = plan.T, plan.k
+    out_dtype = out_dtype or rows.dtype
+    if rows.dim() != 2 or rows.shape[0] != T * k:
+        raise RuntimeError(f"expert_unsort: rows {tuple(rows.shape)} does not have one row per pair of the plan ({T * k})")
+    if rows.dtype not in _CODE or out_dtype not in _CODE or (weights is not None and weights.dtype not in _CODE):
         raise RuntimeError("expert_unsort: rows, weights and the result are float32, bfloat16 or float16")
-    if weights is not None and weights.shape != where.shape:
-        raise RuntimeError(f"expert_unsort: weights {tuple(weights.shape)} must match the plan's {tuple(where.shape)}")
+    if weights is not None and weights.shape != (T, k):
+        raise RuntimeError(f"expert_unsort: weights {tuple(weights.shape)} must match the plan's {(T, k)}")
+    rows = rows.contiguous()
+    weights = None if weights is None else weights.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
-        return _ExpertUnsortFn.apply(rows, weights, where, plan.offsets, out_dtype)
-    if dev.index == torch.cuda.current_device():
-        return _ops().combine(rows, where, weights, out_dtype=out_dtype)
-    with torch.cuda.device(dev):
-        return _ops().combine(rows, where, weights, out_dtype=out_dtype)
+        return _ExpertUnsortFn.apply(rows, weights, plan.planes, T, k, plan.n_experts, out_dtype)
+    return _combine(index, rows, plan.planes.data_ptr(), weights, T, k, out_dtype)
 
 
 # --------------------------------------------------------------------------------------
@@ -216,7 +256,7 @@ def w4_pack(codes, scales, zeros=None) -> W4Weights:
     ``codes`` uint8 [E, N, K/2] (or [N, K/2] for one matrix): two codes a byte, even k in the low nibble; ``scales``
     bfloat16 or float16 [E, N, K/group], ``zeros`` uint8 of the same shape holding 0..15, or None for 8 everywhere.
     ``weight = scale * (code - zero)``.  ``group`` is 32, 64 or 128."""
-    _ready(codes, scales, zeros)
+    index = _ready(codes, scales, zeros)
     if codes.dim() == 2:
         codes, scales = codes.unsqueeze(0), scales.unsqueeze(0)
         zeros = None if zeros is None else zeros.unsqueeze(0)
@@ -241,8 +281,8 @@ def w4_pack(codes, scales, zeros=None) -> W4Weights:
     out_codes = torch.empty((sizes[0],), dtype=torch.uint8, device=dev)
     out_scales = torch.empty((sizes[1] // 2,), dtype=scales.dtype, device=dev)
     out_zeros = None if zeros is None else torch.empty((sizes[2],), dtype=torch.uint8, device=dev)
-    _call(dev, "terrace_w4_pack", codes.data_ptr(), scales.data_ptr(), _hip.ptr(zeros), _hip.float_code(scales.dtype), E, N, K,
-          group, out_codes.data_ptr(), out_scales.data_ptr(), _hip.ptr(out_zeros), _hip.stream(dev))
+    _enqueue(index, "terrace_w4_pack", codes.data_ptr(), scales.data_ptr(), _at(zeros), _CODE[scales.dtype], E, N, K, group,
+             out_codes.data_ptr(), out_scales.data_ptr(), _at(out_zeros))
     return W4Weights(out_codes, out_scales, out_zeros, E, N, K, group, scales.dtype)
 
 
@@ -255,7 +295,7 @@ def expert_linear_w4(rows, tokens_per_expert, weights: W4Weights, swiglu: bool =
     the last expert's give zero rows.  Made for serving, where an expert holds a few rows: the weights are read once per
     16, 32 or 64 rows of an expert.  No gradients: a call that would need them raises."""
     w = weights
-    dev = _ready(rows, tokens_per_expert, w.codes)
+    index = _ready(rows, tokens_per_expert, w.codes)
     if rows.dim() != 2 or rows.shape[1] != w.K or rows.dtype != w.dtype:
         raise RuntimeError(f"expert_linear_w4: rows must be {w.dtype} [P, {w.K}], got {rows.dtype} {tuple(rows.shape)}")
     if tokens_per_expert is None:
@@ -271,10 +311,9 @@ def expert_linear_w4(rows, tokens_per_expert, weights: W4Weights, swiglu: bool =
     rows = _aligned(rows)
     counts = None if tokens_per_expert is None else tokens_per_expert.contiguous()
     P = rows.shape[0]
-    out = torch.empty((P, w.N // 2 if swiglu else w.N), dtype=w.dtype, device=dev)
-    _call(dev, "terrace_w4_linear", rows.data_ptr(), _hip.float_code(w.dtype), P, _hip.ptr(counts), w.codes.data_ptr(),
-          w.scales.data_ptr(), _hip.ptr(w.zeros), w.n_experts, w.N, w.K, w.group, int(swiglu), out.data_ptr(),
-          _hip.stream(dev))
+    out = torch.empty((P, w.N // 2 if swiglu else w.N), dtype=w.dtype, device=w.device)
+    _enqueue(index, "terrace_w4_linear", rows.data_ptr(), _CODE[w.dtype], P, _at(counts), w.codes.data_ptr(),
+             w.scales.data_ptr(), _at(w.zeros), w.n_experts, w.N, w.K, w.group, 1 if swiglu else 0, out.data_ptr())
     return out
 
 
@@ -282,24 +321,23 @@ def expert_linear_w4(rows, tokens_per_expert, weights: W4Weights, swiglu: bool =
 # between two blocks
 # --------------------------------------------------------------------------------------
 
-def _norm_vectors(post_weight, gate, pre_weight, kind):
-    """The (pointer, dtype) arguments of the three vectors, the gate's kind after its own."""
-    def one(v):
-        return (None, 0) if v is None else (v.data_ptr(), _hip.float_code(v.dtype))
-    return (*one(post_weight), *one(gate), kind, *one(pre_weight))
+def _norm_inputs(y, residual, post_weight, gate, kind, pre_weight, scale, eps, T, H):
+    """The arguments that the two entry points share."""
+    y_code = _CODE[residual.dtype if y is None else y.dtype]
+    return (_at(y), y_code, residual.data_ptr(), _CODE[residual.dtype],
+            _at(post_weight), 0 if post_weight is None else _CODE[post_weight.dtype],
+            _at(gate), 0 if gate is None else _CODE[gate.dtype], kind,
+            _at(pre_weight), 0 if pre_weight is None else _CODE[pre_weight.dtype], scale, eps, T, H)
 
 
 def _norm_forward(y, residual, post_weight, gate, kind, pre_weight, scale, eps, want_stats):
     """(h or None, n or None, stats or None) of 2-D packed inputs."""
-    dev = residual.device
     T, H = residual.shape
-    y_dtype = residual.dtype if y is None else y.dtype
     h = None if y is None else torch.empty_like(residual)
-    n = None if pre_weight is None else torch.empty((T, H), dtype=y_dtype, device=dev)
-    stats = torch.empty((T, 2), dtype=torch.float32, device=dev) if want_stats else None
-    _call(dev, "terrace_block_norm", _hip.ptr(y), _hip.float_code(y_dtype), residual.data_ptr(),
-          _hip.float_code(residual.dtype), *_norm_vectors(post_weight, gate, pre_weight, kind), scale, eps, T, H,
-          _hip.ptr(h), _hip.ptr(n), _hip.ptr(stats), _hip.stream(dev))
+    n = None if pre_weight is None else torch.empty_like(residual if y is None else y)
+    stats = torch.empty((T, 2), dtype=torch.float32, device=residual.device) if want_stats else None
+    _enqueue(residual.get_device(), "terrace_block_norm",
+             *_norm_inputs(y, residual, post_weight, gate, kind, pre_weight, scale, eps, T, H), _at(h), _at(n), _at(stats))
     return h, n, stats
 
 
@@ -319,20 +357,18 @@ class _BlockNormFn(torch.autograd.Function):
     def backward(ctx, dh, dn):
         y, residual, post_weight, gate, pre_weight, stats = ctx.saved_tensors
         kind, scale, eps = ctx.norm
-        dev = residual.device
         T, H = residual.shape
         dh, dn = _aligned(dh), _aligned(dn)
-        wanted = [torch.empty_like(t) if t is not None and need else None
+        wanted = [torch.empty_like(t) if need and t is not None else None
                   for t, need in zip((y, residual, post_weight, gate, pre_weight), ctx.needs_input_grad)]
-        d_y, d_residual, d_post, d_gate, d_pre = wanted
-        y_dtype = residual.dtype if y is None else y.dtype
-        need = d_post is not None or d_pre is not None or (d_gate is not None and kind == _hip.GATE_CHANNEL)
-        ws = _hip.workspace(_hip.query("terrace_block_norm_grad_workspace", T, H), dev) if need else None
-        _call(dev, "terrace_block_norm_grad", _hip.ptr(y), _hip.float_code(y_dtype), residual.data_ptr(),
-              _hip.float_code(residual.dtype), *_norm_vectors(post_weight, gate, pre_weight, kind), scale, eps, T, H,
-              stats.data_ptr(), _hip.ptr(dh), _hip.ptr(dn), *(_hip.ptr(t) for t in wanted), _hip.ptr(ws),
-              0 if ws is None else ws.numel(), _hip.stream(dev))
-        return d_y, d_residual, d_post, d_gate, d_pre, None, None, None
+        ws, need = None, 0
+        if wanted[2] is not None or wanted[4] is not None or (wanted[3] is not None and kind == _hip.GATE_CHANNEL):
+            need = _hip.query("terrace_block_norm_grad_workspace", T, H)
+            ws = _hip.workspace(need, residual.device)
+        _enqueue(residual.get_device(), "terrace_block_norm_grad",
+                 *_norm_inputs(y, residual, post_weight, gate, kind, pre_weight, scale, eps, T, H), stats.data_ptr(), _at(dh),
+                 _at(dn), *(_at(t) for t in wanted), _at(ws), need)
+        return (*wanted, None, None, None)
 
 
 def block_norm(y, residual, post_weight=None, gate=None, pre_weight=None, *, scale: float = 1.0, eps: float = 1e-6):
@@ -346,7 +382,8 @@ def block_norm(y, residual, post_weight=None, gate=None, pre_weight=None, *, sca
     the residual may be float32 beside a 16-bit ``y``.  ``h`` has the residual's dtype, ``n`` has ``y``'s; all arithmetic is
     fp32 and each output is rounded once (``n`` comes from the unrounded ``h``).  ``y`` None is the entry of the first
     block: ``h`` is ``residual`` itself and ``n`` its norm.  Carries gradients to all five tensors.  H is at most 16384."""
-    dev = _ready(y, residual, post_weight, gate, pre_weight)
+    tensors = (y, residual, post_weight, gate, pre_weight)
+    _ready(*tensors)
     shape = residual.shape
     if residual.dim() < 1 or (y is not None and y.shape != shape):
         raise RuntimeError(f"block_norm: y and residual must have one shape [..., H], got "
@@ -354,36 +391,40 @@ def block_norm(y, residual, post_weight=None, gate=None, pre_weight=None, *, sca
     if y is None and (post_weight is not None or gate is not None):
         raise RuntimeError("block_norm: post_weight and gate need a y")
     H = shape[-1]
-    if any(t is not None and t.dtype not in _FLOATS for t in (y, residual, post_weight, gate, pre_weight)) or \
-            (y is not None and residual.dtype not in (y.dtype, torch.float32)):
-        raise RuntimeError("block_norm: float32, bfloat16 or float16; the residual of y's dtype or float32")
+    grad = False
+    for t in tensors:
+        if t is not None:
+            if t.dtype not in _CODE:
+                raise RuntimeError(f"block_norm: float32, bfloat16 or float16, got {t.dtype}")
+            grad = grad or t.requires_grad
+    if y is not None and residual.dtype != y.dtype and residual.dtype != torch.float32:
+        raise RuntimeError(f"block_norm: the residual has y's dtype or float32, got {residual.dtype} beside {y.dtype}")
     if not 0 < H <= _MAX_WIDTH:
         raise RuntimeError(f"block_norm: rows of {H} elements; 1 to {_MAX_WIDTH} are taken")
-    for name, v in (("post_weight", post_weight), ("pre_weight", pre_weight)):
-        if v is not None and tuple(v.shape) != (H,):
-            raise RuntimeError(f"block_norm: {name} must be [{H}], got {tuple(v.shape)}")
+    if post_weight is not None and post_weight.shape != (H,):
+        raise RuntimeError(f"block_norm: post_weight must be [{H}], got {tuple(post_weight.shape)}")
+    if pre_weight is not None and pre_weight.shape != (H,):
+        raise RuntimeError(f"block_norm: pre_weight must be [{H}], got {tuple(pre_weight.shape)}")
     kind = _hip.GATE_NONE
     if gate is not None:
-        if tuple(gate.shape) == (H,):
+        if gate.shape == (H,):
             kind = _hip.GATE_CHANNEL
         elif gate.shape == shape[:-1] + (1,):
             kind = _hip.GATE_TOKEN
         else:
             raise RuntimeError(f"block_norm: gate must be [{H}] or {list(shape[:-1]) + [1]}, got {tuple(gate.shape)}")
-    scale, eps = float(scale), float(eps)
     if y is None and pre_weight is None:
         return residual, None
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                           for t in (y, residual, post_weight, gate, pre_weight))
-    flat = residual.dim() != 2
+    scale, eps = float(scale), float(eps)
+    flat = len(shape) != 2
     y2 = y.reshape(-1, H) if flat and y is not None else y
     r2 = residual.reshape(-1, H) if flat else residual
     g2 = gate.reshape(-1, 1) if flat and kind == _hip.GATE_TOKEN else gate
-    args = [_aligned(t) for t in (y2, r2, post_weight, g2, pre_weight)]
-    if grad:
-        h, n = _BlockNormFn.apply(*args, kind, scale, eps)
+    y2, r2, w_post, g2, w_pre = _aligned(y2), _aligned(r2), _aligned(post_weight), _aligned(g2), _aligned(pre_weight)
+    if grad and torch.is_grad_enabled():
+        h, n = _BlockNormFn.apply(y2, r2, w_post, g2, w_pre, kind, scale, eps)
     else:
-        h, n, _ = _norm_forward(args[0], args[1], args[2], args[3], kind, args[4], scale, eps, False)
+        h, n, _ = _norm_forward(y2, r2, w_post, g2, kind, w_pre, scale, eps, False)
     h = residual if y is None else h
     if flat:
         h, n = h.reshape(shape), None if n is None else n.reshape(shape)
