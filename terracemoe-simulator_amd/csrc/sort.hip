@@ -1441,9 +1441,26 @@ int run_hopb_scatter_move(const void *rx, int64_t R, int64_t row_bytes, int quot
 }
 
 // ---- (token, expert) pairs straight to expert order ---------------------------------------------
+// The smallest units that still leave a table for the direct path (no scan launch); without one, make_units' choice.
+// 131072 pairs over 256 experts: four chunks a wave on the direct path, 28 us, where make_units takes sixteen, 47 us.
+static Units expert_units(int64_t P, int n_experts) {
+    for (int c : {1, 4, 16}) {
+        Units u;
+        u.n_items = P;
+        u.n_buckets = n_experts;
+        u.chunks = c;
+        const int64_t units = (P + 64 * c - 1) / (64 * c);
+        if (units > 4096) continue;
+        u.n_units = (int)units;
+        finish_units(u);
+        if (u.direct) return u;
+    }
+    return make_units(P, n_experts);
+}
+
 size_t expert_index_workspace(int64_t P, int n_experts) {
     if (P <= 0 || n_experts <= 0 || n_experts > kMaxBuckets) return 256;
-    return units_table_bytes(make_units(P, n_experts)) + align_up((size_t)P * sizeof(int32_t), 256);
+    return units_table_bytes(expert_units(P, n_experts)) + align_up((size_t)P * sizeof(int32_t), 256);
 }
 
 // The stable sort of P >= 1 pairs by expert: where [P], tokens_per_expert [n_experts] and offsets [n_experts + 1] as
@@ -1452,7 +1469,7 @@ size_t expert_index_workspace(int64_t P, int n_experts) {
 int run_expert_index(const int64_t *expert_idx, int64_t P, int n_experts, int64_t *where, int64_t *tokens_per_expert,
                      int64_t *offsets, int32_t *status, void *ws, const int32_t **pos32, const int32_t **live,
                      hipStream_t s) {
-    const Units u = make_units(P, n_experts);
+    const Units u = expert_units(P, n_experts);
     int32_t *table = (int32_t *)ws;
     int32_t *pos = (int32_t *)((char *)ws + units_table_bytes(u));
     KeyExpert key{expert_idx, n_experts};
