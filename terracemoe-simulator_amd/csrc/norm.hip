@@ -254,21 +254,21 @@ struct NormGrad {
     int want_z, want_v;
 };
 
-template <bool ALIGNED, int E, bool WIDE>
-__device__ __forceinline__ void take_channels(const void *v, int dtype, const float *lds, int64_t H, int at, int tpr,
-                                              float fill, float *f) {
-    if constexpr (WIDE) {
-        load_channels<ALIGNED, E>(v, dtype, H, at, tpr, fill, f);
-    } else {
+// A vector over the channels lies in LDS as two halves, the first and the last four of every piece of eight: neighbouring
+// lanes then read neighbouring 16 bytes.  (Pieces of 32 bytes back to back cost a bank conflict on every read: 1.5e8
+// cycles over the card in a gradient of 16384 rows of 7168, two thirds of its time on every CU.)
+__device__ __forceinline__ int lds_slot(int c, int padded) { return (c & 4 ? padded / 2 : 0) + c / 8 * 4 + c % 4; }
+
+template <int E>
+__device__ __forceinline__ void take_channels(bool given, const float *lds, int padded, int at, int tpr, float fill, float *f) {
 #pragma unroll
-        for (int i = 0; i < E / 8; ++i) {
-            const int c = (at + i * tpr) * 8;
+    for (int i = 0; i < E / 8; ++i) {
+        const int c = (at + i * tpr) * 8;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[i * 8 + j] = fill;
-            if (v && c < H) {                                // whole pieces: the LDS rows are padded to them
+        for (int j = 0; j < 8; ++j) f[i * 8 + j] = fill;
+        if (given && c < padded) {                           // whole pieces: the LDS rows are padded to them
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[i * 8 + j] = lds[c + j];
-            }
+            for (int j = 0; j < 8; ++j) f[i * 8 + j] = lds[lds_slot(c, padded) + j / 4 * (padded / 2) + j % 4];
         }
     }
 }
@@ -276,23 +276,40 @@ __device__ __forceinline__ void take_channels(const void *v, int dtype, const fl
 template <int TY, int TR, bool ALIGNED, int E, bool WIDE>
 __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs a, NormGrad d) {
     __shared__ float part[2][kNormWaves * 3];
-    extern __shared__ float vectors[];                       // [3][H up to a piece]: w_post, gate, w_pre
+    extern __shared__ float vectors[];                       // [2][H up to a piece]: w_post * gate, w_pre
     const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / a.tpr);          // whole waves per row
     const int at = (int)threadIdx.x - group * a.tpr;
     const float inv_h = 1.0f / (float)a.H;
     const int64_t stride = (int64_t)gridDim.x * a.groups;
     const void *channel_gate = a.gate_kind == TERRACE_GATE_CHANNEL ? a.gate : nullptr;
     const int padded = (int)((a.H + 7) / 8 * 8);
-    float *lds_post = vectors, *lds_gate = vectors + padded, *lds_pre = vectors + 2 * padded;
+    const bool has_b = a.w_post || channel_gate;
+    float *lds_b = vectors, *lds_pre = vectors + padded;
     if constexpr (!WIDE) {
         for (int c = threadIdx.x; c < padded; c += blockDim.x) {
             const bool in = c < a.H;
-            if (a.w_post) lds_post[c] = in ? load_scalar(a.w_post, a.post_dtype, c) : 0.0f;
-            if (channel_gate) lds_gate[c] = in ? load_scalar(channel_gate, a.gate_dtype, c) : 0.0f;
-            if (a.w_pre) lds_pre[c] = in ? load_scalar(a.w_pre, a.pre_dtype, c) : 0.0f;
+            float b = in ? 1.0f : 0.0f;
+            if (a.w_post && in) b *= load_scalar(a.w_post, a.post_dtype, c);
+            if (channel_gate && in) b *= load_scalar(channel_gate, a.gate_dtype, c);
+            if (has_b) lds_b[lds_slot(c, padded)] = b;
+            if (a.w_pre) lds_pre[lds_slot(c, padded)] = in ? load_scalar(a.w_pre, a.pre_dtype, c) : 0.0f;
         }
         __syncthreads();
     }
+    // the vectors of this lane's channels: w_post times the gate per channel (the only way they come in), and w_pre
+    auto take = [&](float *b, float *wn) {
+        if constexpr (WIDE) {
+            float g[E];
+            load_channels<ALIGNED, E>(a.w_post, a.post_dtype, a.H, at, a.tpr, 1.0f, b);
+            load_channels<ALIGNED, E>(channel_gate, a.gate_dtype, a.H, at, a.tpr, 1.0f, g);
+            load_channels<ALIGNED, E>(a.w_pre, a.pre_dtype, a.H, at, a.tpr, 0.0f, wn);
+#pragma unroll
+            for (int e = 0; e < E; ++e) b[e] *= g[e];
+        } else {
+            take_channels<E>(has_b, lds_b, padded, at, a.tpr, 1.0f, b);
+            take_channels<E>(a.w_pre != nullptr, lds_pre, padded, at, a.tpr, 0.0f, wn);
+        }
+    };
     float sum[2][WIDE ? 1 : E];
     if constexpr (!WIDE) {
 #pragma unroll
@@ -325,13 +342,11 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
         if constexpr (!WIDE) fetch(row + stride, next);
         float s[3] = {0.0f, 0.0f, 0.0f};
         const float factor = a.scale * cur.token;            // scale, and the token's gate where there is one
-        float wp[E], gc[E], wn[E];
-        take_channels<ALIGNED, E, WIDE>(a.w_post, a.post_dtype, lds_post, a.H, at, a.tpr, 1.0f, wp);
-        take_channels<ALIGNED, E, WIDE>(channel_gate, a.gate_dtype, lds_gate, a.H, at, a.tpr, 1.0f, gc);
-        take_channels<ALIGNED, E, WIDE>(a.w_pre, a.pre_dtype, lds_pre, a.H, at, a.tpr, 0.0f, wn);
+        float b[E], wn[E];
+        take(b, wn);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float u = cur.y.get(e) * cur.inv1, q = gc[e] * (u * wp[e]);
+            const float u = cur.y.get(e) * cur.inv1, q = u * b[e];
             const float h = __fmaf_rn(factor, q, cur.r.get(e)), v = h * cur.inv2, t = cur.dn.get(e) * wn[e];
             s[0] = __fmaf_rn(t, v, s[0]);
             s[1] = __fmaf_rn(__fmaf_rn(cur.inv2, t, cur.dh.get(e)), q, s[1]);
@@ -342,20 +357,18 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
         const float mean_tv = s[0] * inv_h;
         const float dot = __fmaf_rn(-cur.inv2 * mean_tv, s[2], s[1]);         // sum of dH * gate per channel * p
         const float mean_u = factor * dot * inv_h;
-        take_channels<ALIGNED, E, WIDE>(a.w_post, a.post_dtype, lds_post, a.H, at, a.tpr, 1.0f, wp);
-        take_channels<ALIGNED, E, WIDE>(channel_gate, a.gate_dtype, lds_gate, a.H, at, a.tpr, 1.0f, gc);
-        take_channels<ALIGNED, E, WIDE>(a.w_pre, a.pre_dtype, lds_pre, a.H, at, a.tpr, 0.0f, wn);
+        take(b, wn);
         float o1[E], o2[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float u = cur.y.get(e) * cur.inv1;
-            const float h = __fmaf_rn(factor, gc[e] * (u * wp[e]), cur.r.get(e)), v = h * cur.inv2;
+            const float h = __fmaf_rn(factor, u * b[e], cur.r.get(e)), v = h * cur.inv2;
             const float dn = cur.dn.get(e);
             const float dH = __fmaf_rn(cur.inv2, __fmaf_rn(-v, mean_tv, dn * wn[e]), cur.dh.get(e));
             const float z = factor * dH;
             o1[e] = dH;
-            o2[e] = gc[e] * z;
-            if (a.w_post) o2[e] = cur.inv1 * __fmaf_rn(-u, mean_u, o2[e] * wp[e]);
+            o2[e] = z * b[e];
+            if (a.w_post) o2[e] = cur.inv1 * __fmaf_rn(-u, mean_u, o2[e]);
             if constexpr (!WIDE) {
                 sum[0][e] = __fmaf_rn(z, u, sum[0][e]);
                 sum[1][e] = __fmaf_rn(dn, v, sum[1][e]);
@@ -557,7 +570,7 @@ int run_block_norm_grad(const void *y, int y_dtype, const void *residual, int r_
         const NormGrad d{dh, dn, stats, dy, d_residual, gate_kind == TERRACE_GATE_TOKEN ? d_gate : nullptr, (float *)ws, want_z,
                          want_v};
         const unsigned threads = (unsigned)(a.tpr * a.groups);
-        const size_t lds = form.per == 16 ? 0 : (size_t)(3 * ((H + 7) / 8 * 8)) * sizeof(float);
+        const size_t lds = form.per == 16 ? 0 : (size_t)(2 * ((H + 7) / 8 * 8)) * sizeof(float);
 #define TERRACE_NORM(Y, R)                                                                                              \
     if (form.aligned && form.per == 8) block_norm_grad_kernel<Y, R, true, 8, false><<<grid, threads, lds, s>>>(a, d);    \
     else if (form.aligned) block_norm_grad_kernel<Y, R, true, 16, true><<<grid, threads, lds, s>>>(a, d);                \
