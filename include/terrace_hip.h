@@ -520,7 +520,7 @@ TERRACE_API int terrace_expert_unsort_grad(const void *rows, int row_dtype, cons
                                            void *d_weights, terrace_stream_t stream);
 
 /* 4-bit expert weights.  codes [n_experts,N,K/2] bytes (k even in the low nibble), scales [n_experts,N,K/group] of dtype
- * (BF16 or F16), zeros [n_experts,N,K/group] bytes 0..15 or NULL (8 everywhere): weight = scale * (code - zero).  group is 32, 64
+ * (BF16 or F16), zeros [n_experts,N,K/group] bytes whose low four bits count, or NULL (8 everywhere): weight = scale * (code - zero).  group is 32, 64
  * or 128 and divides K.  terrace_w4_pack lays them out for terrace_w4_linear, once per weight; terrace_w4_packed_bytes
  * tells the size of each packed plane (what: 0 codes, 1 scales, 2 zeros; 0 bytes: a shape that is not taken). */
 TERRACE_API size_t terrace_w4_packed_bytes(int n_experts, int64_t N, int64_t K, int group, int what);

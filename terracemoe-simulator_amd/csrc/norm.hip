@@ -482,7 +482,7 @@ static int norm_check(const NormArgs &a, int y_dtype, int r_dtype) {
     if (a.T < 0 || a.H <= 0 || a.H > kNormMaxH || !norm_float(y_dtype) || !norm_float(r_dtype) ||
         (r_dtype != y_dtype && r_dtype != TERRACE_F32) || a.gate_kind < TERRACE_GATE_NONE || a.gate_kind > TERRACE_GATE_TOKEN ||
         (a.T > 0 && (a.gate_kind != TERRACE_GATE_NONE) != (a.gate != nullptr)) || (a.w_post && !norm_float(a.post_dtype)) ||
-        (a.gate && !norm_float(a.gate_dtype)) || (a.w_pre && !norm_float(a.pre_dtype)) || a.T >= ((int64_t)1 << 22) ||
+        (a.gate && !norm_float(a.gate_dtype)) || (a.w_pre && !norm_float(a.pre_dtype)) ||
         (a.T > 0 && !a.y && (a.w_post || a.gate)))
         return TERRACE_EINVAL;
     return TERRACE_OK;

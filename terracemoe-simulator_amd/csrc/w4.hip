@@ -124,7 +124,9 @@ __global__ __launch_bounds__(kBlock) void w4_pack_groups_kernel(const V *__restr
         const int64_t g = rest % sh.blocks() * gpb + d % gpb;
         rest /= sh.blocks();
         const int64_t n = rest % sh.tiles() * kTileN + col, e = rest / sh.tiles();
-        packed[d] = n < sh.N && g < groups ? plane[(e * sh.N + n) * groups + g] : V(0);
+        V v = n < sh.N && g < groups ? plane[(e * sh.N + n) * groups + g] : V(0);
+        if (sizeof(V) == 1) v &= 15;                         // a zero point has four bits: more would reach the exponent
+        packed[d] = v;
     }
 }
 

@@ -88,6 +88,8 @@ class ExpertPlan:
     __slots__ = ("planes", "T", "k", "n_experts", "_made")
 
     def __init__(self, planes, T, k, n_experts):
+        if planes.dtype != torch.int64 or planes.numel() != self.words(T, k, n_experts) or not planes.is_contiguous():
+            raise RuntimeError("ExpertPlan: the planes do not match the geometry")
         self.planes, self.T, self.k, self.n_experts, self._made = planes, T, k, n_experts, {}
 
     @staticmethod
@@ -121,14 +123,17 @@ class ExpertPlan:
 def _sort_raw(index, x, expert_idx, planes, T, k, n):
     x = _movable_rows(x)
     expert_idx = expert_idx.contiguous()
-    rows = torch.empty((T * k, x.shape[1]), dtype=x.dtype, device=x.device) if x.is_contiguous() else \
-        _hip.empty_rows(T * k, x)
+    if x.is_contiguous():
+        rows, row_bytes = torch.empty((T * k, x.shape[1]), dtype=x.dtype, device=x.device), x.shape[1] * x.element_size()
+    else:
+        rows, row_bytes = _hip.empty_rows(T * k, x), _hip.row_arg(x)
     need = _hip.query("terrace_expert_sort_workspace", T, k, n)
     ws = _hip.workspace(need, x.device) if need > 256 else None      # 256: the one-launch form, which needs none
     base = planes.data_ptr()
     counts = base + 8 * T * k
-    _enqueue(index, "terrace_expert_sort", x.data_ptr(), expert_idx.data_ptr(), T, _hip.row_arg(x), k, n, rows.data_ptr(),
-             base, counts, counts + 8 * n, counts + 8 * (2 * n + 1), _at(ws), need if ws is not None else 0)
+    src, dst = (x.data_ptr(), rows.data_ptr()) if rows.numel() else (None, None)
+    _enqueue(index, "terrace_expert_sort", src, expert_idx.data_ptr(), T, row_bytes, k, n, dst, base, counts,
+             counts + 8 * n, counts + 8 * (2 * n + 1), _at(ws), need if ws is not None else 0)
     return rows
 
 
@@ -254,7 +259,8 @@ def w4_pack(codes, scales, zeros=None) -> W4Weights:
     """Lay 4-bit weights out for :func:`expert_linear_w4`, once per weight; the inputs may be freed afterwards.
 
     ``codes`` uint8 [E, N, K/2] (or [N, K/2] for one matrix): two codes a byte, even k in the low nibble; ``scales``
-    bfloat16 or float16 [E, N, K/group], ``zeros`` uint8 of the same shape holding 0..15, or None for 8 everywhere.
+    bfloat16 or float16 [E, N, K/group], ``zeros`` uint8 of the same shape (the low four bits count), or None for 8
+    everywhere.
     ``weight = scale * (code - zero)``.  ``group`` is 32, 64 or 128."""
     index = _ready(codes, scales, zeros)
     if codes.dim() == 2:

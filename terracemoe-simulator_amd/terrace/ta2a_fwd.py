@@ -395,6 +395,31 @@ def ta2a_loopback_forward(x, expert_idx, gates, expert_fn, world: int, n_experts
     return loopback_combine(ye, st), st
 
 
+def local_forward(x, expert_idx, gates, expert_fn, n_experts: int):
+    """sort -> ``expert_fn(rows, tokens_per_expert) -> ye`` -> weighted way back, when every expert lives on this GPU:
+    what :func:`ta2a_loopback_forward` computes, without the hops and without its equal-quota condition (any routing,
+    pairs without an expert included), and differentiable: gradients reach ``x``, ``gates`` and, through ``expert_fn``,
+    the experts.  A token's rows are added in the order of its columns; with ascending expert ids that is
+    :func:`loopback_combine`'s order and the results agree bit for bit.  Returns ``(y, plan)``."""
+    rows, plan = _ops.expert_sort(x, expert_idx, n_experts)
+    ye = expert_fn(rows, plan.tokens_per_expert)
+    return _ops.expert_unsort(ye, gates, plan), plan
+
+
+def w4_experts(w_in, w_out):
+    """An ``expert_fn`` for :func:`local_forward` and :func:`ta2a_loopback_forward` (drop-less): the feed-forward experts
+    ``w_out . (silu(gate) * up)`` on 4-bit weights (``ops.w4_pack``), ``w_in`` [E, 2I, H] holding the gate's rows and
+    then the up projection's, ``w_out`` [E, H, I].  Forward only."""
+    if w_in.N % 2 or w_out.K != w_in.N // 2 or w_in.n_experts != w_out.n_experts or w_in.dtype != w_out.dtype:
+        raise RuntimeError(f"w4_experts: {w_in.n_experts} x [{w_in.N}, {w_in.K}] {w_in.dtype} cannot feed "
+                           f"{w_out.n_experts} x [{w_out.N}, {w_out.K}] {w_out.dtype}")
+
+    def experts(rows, tokens_per_expert):
+        mid = _ops.expert_linear_w4(rows, tokens_per_expert, w_in, swiglu=True)
+        return _ops.expert_linear_w4(mid, tokens_per_expert, w_out)
+    return experts
+
+
 def ta2a_moe_forward(*_args, **_kwargs):
     raise NotImplementedError("ta2a_moe_forward needs the all-to-all exchanges of a multi-GPU run; this "
                               "one-GPU build provides ta2a_loopback_forward and the per-stage operators")

@@ -552,12 +552,10 @@ def test_refusals():
 # ---- together -----------------------------------------------------------------------------------------------------
 def moe_block(tops, terrace, x, cfg, logits, bias, w_in, w_out, pre, post, gate, nxt):
     """One serving block: the norm before, the route, tokens to expert order, the experts, and back."""
+    from terrace.ta2a_fwd import local_forward, w4_experts
     h0, n0 = tops.block_norm(None, x, pre_weight=pre)
     idx, gates, _ = terrace.t_route(logits, bias, cfg, gates_dtype=x.dtype)
-    rows, plan = tops.expert_sort(n0, idx, cfg.n_experts)
-    mid = tops.expert_linear_w4(rows, plan.tokens_per_expert, w_in, swiglu=True)
-    out = tops.expert_linear_w4(mid, plan.tokens_per_expert, w_out)
-    y = tops.expert_unsort(out, gates, plan)
+    y, _ = local_forward(n0, idx, gates, w4_experts(w_in, w_out), cfg.n_experts)
     return tops.block_norm(y, h0, post, gate, nxt, scale=0.5)
 
 
@@ -625,6 +623,182 @@ def test_a_block_of_them_together_and_as_a_graph(T):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(gh, eh) and torch.equal(gn, en)
+
+
+def test_the_local_path_is_the_loopback_path_without_its_hops():
+    import terrace.ops as tops
+    from conftest import equal_quota_routing
+    from terrace.ta2a_fwd import local_forward, ta2a_loopback_forward, w4_experts
+    announce("local against loopback")
+    T, E, k, M, H, I = 500, 32, 4, 2, 128, 64
+    idx = torch.from_numpy(equal_quota_routing(T, k, E, 4, M, 3, sort_rows=True)).to(DEV)       # 4 nodes of 8 cards
+    g = gen(4)
+    x = torch.randn((T, H), generator=g, device=DEV).bfloat16()
+    gates = torch.rand((T, k), generator=g, device=DEV).bfloat16()
+    ci, si, _, _, _ = w4_case(E, 2 * I, H, 64, "bf16", False, 1)
+    co, so, _, _, _ = w4_case(E, H, I, 64, "bf16", False, 2)
+    # every node of the loop-back holds its own 8 experts' slots: the same 8 matrices on each
+    ci, si, co, so = (t[:8].repeat(4, 1, 1) for t in (ci, si, co, so))
+    here, _ = local_forward(x, idx, gates, w4_experts(tops.w4_pack(ci, si), tops.w4_pack(co, so)), E)
+    slots = w4_experts(tops.w4_pack(ci[:8], si[:8]), tops.w4_pack(co[:8], so[:8]))
+    there, _ = ta2a_loopback_forward(x, idx, gates, slots, 32, E, 8, M)
+    assert torch.equal(here, there)
+
+
+def test_the_local_path_trains():
+    """Gradients of x, the gates and the experts' weights through sort, experts and the way back, against autograd of the
+    same layer in 64 bits: f32 products of 32 and 4 terms and 200 rows, so 2^-24 times a few hundred of the terms."""
+    from terrace.ta2a_fwd import local_forward
+    announce("local trains")
+    T, E, k, H = 200, 6, 3, 32
+    idx = routing(T, E, k, 8, 0.2)
+    g = gen(12)
+    x = torch.randn((T, H), generator=g, device=DEV, requires_grad=True)
+    gates = torch.rand((T, k), generator=g, device=DEV, requires_grad=True)
+    w = (torch.randn((E, H), generator=g, device=DEV) / 4).requires_grad_(True)
+    dy = torch.randn((T, H), generator=g, device=DEV)
+
+    def experts(rows, counts):                               # a scale per expert and channel, from the counts alone
+        ends = torch.cumsum(counts, 0)
+        e = torch.searchsorted(ends, torch.arange(rows.shape[0], device=DEV), right=True).clamp(max=E - 1)
+        return rows * w[e]
+
+    y, plan = local_forward(x, idx, gates, experts, E)
+    got = torch.autograd.grad(y, (x, gates, w), dy)
+    xd, gd, wd = (t.detach().double().requires_grad_(True) for t in (x, gates, w))
+    live = (idx >= 0).double()
+    yd = ((gd * live)[..., None] * (xd[:, None, :] * wd[idx.clamp(min=0)])).sum(1)
+    want = torch.autograd.grad(yd, (xd, gd, wd), dy.double())
+    near(y, yd.detach(), (gd.abs()[..., None] * (xd.abs()[:, None, :] * wd.abs()[idx.clamp(min=0)])).sum(1).detach(), 3 * k, "y")
+    size = [((gd.abs() * live)[..., None] * wd.abs()[idx.clamp(min=0)] * dy.double().abs()[:, None]).sum(1).detach(),
+            (live[..., None] * (xd.abs()[:, None] * wd.abs()[idx.clamp(min=0)] * dy.double().abs()[:, None])).sum(2).detach()]
+    terms = ((gd.abs() * live)[..., None] * xd.abs()[:, None] * dy.double().abs()[:, None]).detach()
+    size.append(torch.zeros((E, H), dtype=torch.float64, device=DEV).index_add_(0, idx.clamp(min=0).reshape(-1),
+                                                                                terms.reshape(-1, H)))
+    for name, a, b, m, chain in zip(("x", "gates", "experts"), got, want, size, (3 * k, 2 * H, 3 * T * k)):
+        near(a, b, m, chain, name)
+
+
+@pytest.mark.parametrize("T", [40, 1200])
+def test_a_training_step_as_a_graph(T):
+    """Forward and backward of all the differentiable operators recorded once and replayed on new inputs, with eager work
+    between the replays: every replay gives the eager step's bits."""
+    import terrace.ops as tops
+    announce("training graph", T)
+    E, k, H = 8, 3, 264
+    g = gen(T)
+
+    def normal(s, a=1.0, b=0.0):
+        return (torch.randn(s, generator=g, device=DEV) * a + b).bfloat16()
+
+    x, gates, idx = normal((T, H)), normal((T, k), 0.2, 0.5), routing(T, E, k, T, 0.2)
+    vec = [normal((H,), 0.1, 1.0) for _ in range(3)]
+    up = [normal((T, H)), normal((T, H))]
+    for t in (x, gates, *vec):
+        t.requires_grad_(True)
+
+    def step():
+        h0, n0 = tops.block_norm(None, x, pre_weight=vec[0])
+        rows, plan = tops.expert_sort(n0, idx, E)
+        y = tops.expert_unsort(rows, gates, plan)
+        h, n = tops.block_norm(y, h0, vec[1], None, vec[2], scale=0.5)
+        return (h.detach(), n.detach(), *torch.autograd.grad((h, n), (x, gates, *vec), up))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for rep in range(3):
+        announce("training graph", T, rep)
+        with torch.no_grad():
+            x.copy_(normal((T, H)))
+            gates.copy_(normal((T, k), 0.2, 0.5))
+            idx.copy_(routing(T, E, k, T + rep + 1, 0.2))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_buffers_beyond_four_gigabytes():
+    """Offsets past 2^32 bytes in every operator, rows from all over the buffers against the plain formulas."""
+    import terrace.ops as tops
+    T, H = 300_000, 8192
+    announce("large block_norm", T, H)
+    g = gen(1)
+    y = torch.randn((T, H), generator=g, device=DEV, dtype=torch.bfloat16)
+    r = torch.randn((T, H), generator=g, device=DEV, dtype=torch.bfloat16)
+    w = torch.ones((H,), device=DEV, dtype=torch.bfloat16)
+    pick = torch.tensor([0, 1, 131_072, 262_143, 262_144, T - 1], device=DEV)
+    y.requires_grad_(True)
+    h, n = tops.block_norm(y, r, w, None, w)
+    (dy,) = torch.autograd.grad((h, n), y, (r, r))
+    val, mag = norm_oracle(y.detach()[pick], r[pick], w, None, w, 1.0, 1e-6, r[pick], r[pick])
+    for name, got in (("h", h), ("n", n), ("d_y", dy)):
+        near(got.detach()[pick], val[name], mag[name], H / 64 + 40, name)
+    del h, n, dy, y, r
+    announce("large expert_sort")
+    T, k, H, E = 40_000, 8, 8192, 64                         # 320000 rows of 16 KB
+    x = torch.randn((T, H), generator=g, device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+    idx = routing(T, E, k, 5)
+    rows, plan = tops.expert_sort(x, idx, E)
+    where, counts, offsets = sort_oracle(idx, E)
+    assert torch.equal(plan.where.cpu(), where)
+    at = plan.where[pick[:2].tolist() + [T - 1]]
+    assert torch.equal(rows[at.reshape(-1)], x[pick[:2].tolist() + [T - 1]].repeat_interleave(k, 0))
+    gates = torch.rand((T, k), generator=g, device=DEV).bfloat16().requires_grad_(True)
+    yy = tops.expert_unsort(rows, gates, plan)
+    dx, dg = torch.autograd.grad(yy, (x, gates), x.detach())
+    tok = torch.tensor([0, T // 2, T - 1], device=DEV)
+    xd, gd = x.detach()[tok].double(), gates.detach()[tok].double()
+    near(yy.detach()[tok], xd * gd.sum(1, keepdim=True), xd.abs() * gd.sum(1, keepdim=True), 2 * k, "y")
+    # the gradient of the rows is rounded before the sort's gradient adds the k of a token: half a bf16 step of each term
+    terms = gd[:, :, None] * xd[:, None, :]
+    assert bool(((dx[tok].double() - terms.sum(1)).abs() <= 2.0 ** -8 * 1.01 * (terms.abs().sum(1) + terms.sum(1).abs())).all())
+    dots = (xd * xd).sum(1, keepdim=True).expand(-1, k)
+    near(dg[tok], dots, dots, H / 256 + 20, "d_gates")
+    del rows, yy, dx, dg, x
+    announce("large w4")
+    E, N, K = 300, 4096, 7168                                # 4.4 GB of codes
+    codes = torch.randint(0, 256, (E, N, K // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = torch.full((E, N, K // 128), 0.01, device=DEV, dtype=torch.bfloat16)
+    packed = tops.w4_pack(codes, scales)
+    counts = torch.zeros((E,), dtype=torch.int64, device=DEV)
+    counts[0], counts[E - 2], counts[E - 1] = 1, 1, 2
+    x = torch.randn((4, K), generator=g, device=DEV).bfloat16()
+    out = tops.expert_linear_w4(x, counts, packed)
+    for row, e in enumerate((0, E - 2, E - 1, E - 1)):
+        q = torch.stack((codes[e] & 15, codes[e] >> 4), -1).flatten(-2).double()
+        s = float(scales[0, 0, 0])
+        near(out[row], (q - 8) @ x[row].double() * s, (q + 40) @ x[row].double().abs() * s, 2 * 130 + K / 128 + 10, f"row {row}")
+
+
+def test_w4_zero_points_count_with_their_low_four_bits():
+    import terrace.ops as tops
+    announce("w4 zeros")
+    codes, scales, z, _, _ = w4_case(2, 40, 128, 32, "bf16", True, 3)
+    x = torch.randn((5, 128), generator=gen(1), device=DEV).bfloat16()
+    counts = torch.tensor([2, 3], device=DEV)
+    assert torch.equal(tops.expert_linear_w4(x, counts, tops.w4_pack(codes, scales, z)),
+                       tops.expert_linear_w4(x, counts, tops.w4_pack(codes, scales, z | 0xB0)))
+
+
+def test_expert_sort_rows_without_width():
+    import terrace.ops as tops
+    announce("no width")
+    idx = routing(30, 8, 2, 1)
+    wide = torch.randn((30, 16), generator=gen(1), device=DEV)
+    rows, plan = tops.expert_sort(wide[:, :0], idx, 8)
+    assert rows.shape == (60, 0) and torch.equal(plan.where.cpu(), sort_oracle(idx, 8)[0])
+    with pytest.raises(RuntimeError, match="geometry"):
+        tops.ExpertPlan(plan.planes, 31, 2, 8)
 
 
 def test_two_streams_at_once():
