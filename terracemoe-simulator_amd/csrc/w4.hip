@@ -190,27 +190,33 @@ __device__ __forceinline__ int wave_scan(int v, int most) {
 __device__ __forceinline__ RowTile find_tile(const int64_t *__restrict__ counts, int n_experts, int P, int R, int tile) {
     const int lane = lane_id();
     int rows = 0, tiles = 0;                                 // before the experts looked at
-    auto count = [&](int e) { return e >= n_experts ? (int64_t)0 : counts ? counts[e] : (int64_t)P; };
-    int64_t c = count(lane);
-    for (int e0 = 0; e0 < n_experts; e0 += kWave) {
-        const int64_t now = c;
-        c = count(e0 + kWave + lane);
-        const int n = now < 0 ? 0 : now > P ? P : (int)now;
-        int upto = wave_scan(n, P) + rows;
-        if (upto > P) upto = P;
-        int from = __shfl_up(upto, 1, kWave);
-        if (lane == 0) from = rows;
-        const int mine = (upto - from + R - 1) / R;
-        const int upto_tiles = wave_scan(mine, P) + tiles;
-        const uint64_t past = __ballot(upto_tiles > tile);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            const int skip = (tile - read_lane(upto_tiles - mine, at)) * R;
-            const int first = read_lane(from, at), n_rows = read_lane(upto, at) - first - skip;
-            return {e0 + at, first + skip, n_rows < R ? n_rows : R, 0, 0};
+    constexpr int kLoads = 4;                                // 256 experts' counts in flight at once
+    for (int e0 = 0; e0 < n_experts; e0 += kLoads * kWave) {
+        int64_t c[kLoads];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int e = e0 + j * kWave + lane;
+            c[j] = e >= n_experts ? 0 : counts ? counts[e] : P;
         }
-        rows = read_lane(upto, kWave - 1);
-        tiles = read_lane(upto_tiles, kWave - 1);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int n = c[j] < 0 ? 0 : c[j] > P ? P : (int)c[j];
+            int upto = wave_scan(n, P) + rows;
+            if (upto > P) upto = P;
+            int from = __shfl_up(upto, 1, kWave);
+            if (lane == 0) from = rows;
+            const int mine = (upto - from + R - 1) / R;
+            const int upto_tiles = wave_scan(mine, P) + tiles;
+            const uint64_t past = __ballot(upto_tiles > tile);
+            if (past) {
+                const int at = __builtin_ctzll(past);
+                const int skip = (tile - read_lane(upto_tiles - mine, at)) * R;
+                const int first = read_lane(from, at), n_rows = read_lane(upto, at) - first - skip;
+                return {e0 + j * kWave + at, first + skip, n_rows < R ? n_rows : R, 0, 0};
+            }
+            rows = read_lane(upto, kWave - 1);
+            tiles = read_lane(upto_tiles, kWave - 1);
+        }
     }
     return {-1, 0, 0, tiles, rows};
 }
