@@ -19,13 +19,15 @@ int run_expert_index(const int64_t *expert_idx, int64_t P, int n_experts, int64_
 // ---------------------------------------------------------------------------------------------
 // few pairs: one launch
 // ---------------------------------------------------------------------------------------------
-// Up to kSmallPairs pairs the place of a pair is found by comparing it with every other one: with key(p) = expert of p
+// With few pairs the place of a pair is found by comparing it with every other one: with key(p) = expert of p
 // (n_experts for a pair without one) and code(p) = key(p) * P + p, place(p) = #{p' : code(p') < code(p)}.  Every
 // workgroup does that for the k pairs of its own token -- P * k compares, one ballot per 64 of them -- and then moves its
 // slice of the token's row; a pair without an expert ranks behind all others, so its place is one of the rows behind
 // the live ones and the workgroup writes zeros there.  The last workgroup writes the counts.  No workspace, no second
 // launch: what bounds it is the latency of one launch and two dependent reads (the ids, then nothing but stores).
-constexpr int64_t kSmallPairs = 2048;
+// 8 experts of 256 a token, 14 KB rows, against the sorting path: 32 tokens 4.7 us for 9.8, 128 tokens 7.9 for 10.9, 512
+// tokens 26 for 35, 1024 tokens 62 for 48; one expert a token, 2000 tokens 10.3 for 19.2, 8000 tokens 66 for 17.
+static bool few_pairs(int64_t T, int64_t P) { return P <= 2048 || (P <= 4096 && T <= 1024); }
 constexpr int kMaxSmallExperts = kMaxBuckets;
 constexpr int kSmallFan = 16;
 
@@ -138,7 +140,7 @@ static int row_vec_bytes(const RowGeom &g, const void *a, const void *b) {
 }
 
 size_t expert_sort_workspace(int64_t T, int k, int n_experts) {
-    if (T <= 0 || k <= 0 || T > (((int64_t)1 << 31) - 1) / k || T * k <= kSmallPairs) return 256;
+    if (T <= 0 || k <= 0 || T > (((int64_t)1 << 31) - 1) / k || few_pairs(T, T * k)) return 256;
     return expert_index_workspace(T * k, n_experts);
 }
 
@@ -158,7 +160,7 @@ int run_expert_sort(const void *x, const int64_t *expert_idx, int64_t T, int64_t
     if (x && g.pitched() && (((uintptr_t)x | (uintptr_t)rows) & 15)) return TERRACE_EINVAL;
     const bool move = x && g.width > 0;
     const int vb = move ? row_vec_bytes(g, x, rows) : 16;
-    if (P <= kSmallPairs) {
+    if (few_pairs(T, P)) {
         const int64_t vecs = move ? g.width / vb : 1;
         const int64_t slices = (vecs + kBlock - 1) / kBlock;
         if (T * slices >= ((int64_t)1 << 31) / kBlock) return TERRACE_EINVAL;

@@ -170,8 +170,8 @@ def expert_sort(x, expert_idx, n_experts: int):
     -- and one past ``n_experts`` is treated the same and reported in ``plan.status``; such a pair has ``where`` -1, and
     the rows behind the last live one are zeros.  A token may have no expert at all.  ``rows`` carries gradients to ``x``
     (any dtype may be sorted; gradients need float32, bfloat16 or float16).  ``plan.tokens_per_expert`` is what
-    :func:`expert_linear_w4` takes, ``plan.where`` what ``combine`` takes.  At most 2048 experts.  Up to 2048 pairs the
-    call is one launch."""
+    :func:`expert_linear_w4` takes, ``plan.where`` what ``combine`` takes.  At most 2048 experts.  Up to 2048 pairs (4096
+    over at most 1024 tokens) the call is one launch."""
     index = _ready(x, expert_idx)
     if x.dim() != 2 or expert_idx.dim() != 2 or x.shape[0] != expert_idx.shape[0]:
         raise RuntimeError(f"expert_sort: x {tuple(x.shape)} and expert_idx {tuple(expert_idx.shape)} must be [T, H] "

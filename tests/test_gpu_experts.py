@@ -78,7 +78,7 @@ def check_sort(x, idx, E):
 @pytest.mark.parametrize("T,E,k,H,dtype,dead", [
     (0, 8, 2, 16, "bf16", 0.0), (1, 1, 1, 1, "f32", 0.0), (1, 256, 8, 7168, "bf16", 0.0), (1, 8, 2, 5, "f16", 1.0),
     (61, 128, 8, 4096, "bf16", 0.25), (64, 2048, 8, 40, "f32", 0.1), (3, 4, 17, 24, "bf16", 0.3), (2, 5, 40, 9, "f16", 0.3),
-    (256, 8, 8, 33, "bf16", 0.0), (257, 8, 8, 33, "bf16", 0.2), (2048, 7, 1, 64, "f32", 0.5), (2049, 7, 1, 64, "f32", 0.5),
+    (256, 8, 8, 33, "bf16", 0.0), (257, 8, 8, 33, "bf16", 0.2), (1024, 2048, 4, 24, "bf16", 0.1), (1025, 9, 4, 24, "bf16", 0.1), (2048, 7, 1, 64, "f32", 0.5), (2049, 7, 1, 64, "f32", 0.5),
     (4096, 64, 4, 128, "f32", 0.0), (5003, 60, 6, 72, "bf16", 0.1), (3000, 2048, 8, 16, "f16", 0.2),
     (700, 300, 3, 7, "bf16", 1.0), (9000, 256, 8, 520, "bf16", 0.05),
 ])
