@@ -272,6 +272,8 @@ def check_w4(E, N, K, group, dtype, zeros, swiglu, counts, tail=0, seed=0):
     (1, 256, 1024, 128, False, False, [1]), (3, 80, 160, 32, True, False, [64, 65, 63]),
     (2, 11000, 160, 32, True, True, [130, 40]), (3, 20000, 128, 128, False, False, [20, 33, 1]), (1, 16400, 96, 32, False, True, [250]),
     (2, 24010, 448, 64, True, False, [64, 64]), (1, 66000, 32, 32, False, False, [33]),
+    (1, 50, 640, 128, True, True, [100]), (1, 40, 1120, 32, False, False, [31]), (2, 66, 2048, 64, True, False, [130, 3]),
+    (1, 130, 416, 32, True, False, [64]),
 ])
 def test_w4_products(E, N, K, group, zeros, swiglu, counts, dtype):
     check_w4(E, N, K, group, dtype, zeros, swiglu, counts, 0, E + N)
