@@ -385,14 +385,14 @@ __device__ __forceinline__ void w4_use(W4Block<T, 4 / GS, ZEROS> &k, X x, f32x4 
 
 __device__ __forceinline__ float w4_swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
 
-// Few rows: tiles of 16.  One token through the gate and up projections of 8 experts (117 MB of codes) 24.7 us, 512 rows over
-// 256 experts of 7168 x 2048 230 us at 6.8-7 TB/s: the HBM bytes of the codes, behind about 5 us of launch, look-up and
-// first load.  A set of 32 columns -- two tiles: neighbours, or with `swiglu` the same columns of both halves --
-// is the work of `split` waves that share out the blocks of k and are joined in LDS, in order; a workgroup holds 4 or 8
+// Few rows: tiles of 16.  One token through the gate and up projections of 8 experts (121 MB) 25 us, 4.8 TB/s; 512 rows
+// over 174 busy experts of 7168 x 2048 (1.33 GB) 245 us, 5.4 TB/s, with vector instructions in 45 % of the cycles.  A set of
+// 32 columns -- two tiles: neighbours, or with `swiglu` the same columns of both halves -- is the work of `split` waves that share out the blocks of k and are joined in LDS, in order; a workgroup holds 4 or 8
 // waves and so 4 / split or 8 / split sets.  The rows' fragments come straight from memory (a few rows: L1 and L2), and
 // codes and rows are fetched kAhead blocks ahead, because the codes come from HBM and nothing else hides their latency.
-// (One token: 27.7 us with two blocks ahead, 28.4 with three, 31.1 with four, whose registers cost waves.  4096 waves or more
-// fill the card: sharing k out further for one token 30.4 us, for one down projection 22.3 for 17.2.)
+// (One token, measured before the codes were loaded around the cache: 27.8 us with two blocks ahead, 31.1 with four, whose
+// registers cost waves; k shared out among up to 8192 waves and not 4096 30.4 us for 27.8, one token's down projection
+// 22.3 for 17.2.)
 constexpr int kAhead = 2;
 constexpr int kMaxSplit = 8;
 
@@ -493,9 +493,10 @@ __global__ __launch_bounds__(kMaxSplit * kWave) void w4_few_kernel(W4Args a) {
 // Tens of rows: tiles of 16 * MT.  A workgroup of four waves makes 256 columns, each wave four tiles (with `swiglu` two of
 // each half), so the rows of a block of k are read once for 256 columns: they go through LDS in the order the matrix
 // instructions take them, while every wave streams its own codes two blocks ahead.  2048 rows over 64 experts of 4096 x
-// 4096 199 us (0.34 PFLOP/s, 3.1 TB/s of codes), 256 rows of each of 8 experts 86 us: bound by vector instructions, about
-// 320 for the 40 matrix instructions of a block and wave (112 expand codes, 128 scale each group's sums).  From more than
-// 8 rows a busy expert on it beats the kernel above: 1024 rows over 64 experts 138 us for 194.
+// 4096 199-211 us (0.33 PFLOP/s, 612 MB), 256 rows of each of 8 experts 85-90 us.  By counters vector instructions (307 a block
+// and wave, and the issue of 40 matrix instructions) fill 60 % of the cycles and matrix instructions 28 %: neither is full, and two
+// waves a SIMD do not hide one behind the other.  From more than 8 rows a busy expert on it beats the kernel above: 1024
+// rows over 64 experts of 2048 x 7168 141 us for 194.
 constexpr int kManyTiles = 4;
 // (two waves a SIMD at least: with a whole SIMD's registers to itself the compiler puts the sums into accumulation
 // registers and copies each out again before the multiply-add, a fifth of the kernel's instructions)
