@@ -818,3 +818,94 @@ def test_two_streams_at_once():
                 got[i].append(tops.expert_sort(x[i], idx[i], 16)[0])
     torch.cuda.synchronize()
     assert all(torch.equal(r, want[i]) for i in range(2) for r in got[i])
+
+
+def off_boundary(t):
+    """The values of ``t``, packed, starting one element behind a 16-byte boundary."""
+    flat = torch.empty((t.numel() + 8,), dtype=t.dtype, device=DEV)
+    view = flat[1:1 + t.numel()].view(t.shape)
+    view.copy_(t)
+    assert view.is_contiguous() and view.data_ptr() % 16
+    return view
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_the_sort_and_back_off_a_16_byte_boundary(dtype):
+    import terrace.ops as tops
+    announce("off boundary", dtype)
+    T, E, k, H = 70, 9, 3, 64
+    g = gen(31)
+    idx = off_boundary(routing(T, E, k, 32, 0.2))
+    check_sort(off_boundary(torch.randn((T, H), generator=g, device=DEV).to(DT[dtype])), idx, E)
+    _, plan = tops.expert_sort(torch.zeros((T, 8), device=DEV), idx, E)
+    rows = off_boundary(torch.randn((T * k, H), generator=g, device=DEV).to(DT[dtype])).requires_grad_(True)
+    weights = off_boundary(torch.rand((T, k), generator=g, device=DEV).to(DT[dtype])).requires_grad_(True)
+    dy = off_boundary(torch.randn((T, H), generator=g, device=DEV).to(DT[dtype]))
+    want_y, mag_y, want_rows, want_w, mag_w = unsort_oracle(rows.detach(), weights.detach(), plan, dy)
+    y = tops.expert_unsort(rows, weights, plan)
+    near(y, want_y, mag_y, 2 * k, "y")
+    d_rows, d_w = torch.autograd.grad(y, (rows, weights), dy)
+    near(d_rows, want_rows, want_rows.abs(), 1, "d_rows")
+    near(d_w, want_w, mag_w, H / 64 + 8 + 10, "d_weights")
+
+
+def test_gradients_that_arrive_expanded():
+    import terrace.ops as tops
+    announce("expanded gradients")
+    T, E, k, H = 40, 6, 2, 72
+    g = gen(41)
+    idx = routing(T, E, k, 42, 0.3)
+    x = torch.randn((T, H), generator=g, device=DEV).requires_grad_(True)
+    w = torch.rand((T, k), generator=g, device=DEV).requires_grad_(True)
+    gain = torch.rand((H,), generator=g, device=DEV).requires_grad_(True)
+
+    def leaves(expanded):
+        rows, plan = tops.expert_sort(x, idx, E)
+        h, n = tops.block_norm(tops.expert_unsort(rows, w, plan), x, None, None, gain)
+        one = torch.ones((), device=DEV).expand(T, H)
+        d = one if expanded else one.contiguous()
+        direct = torch.autograd.grad(rows, x, torch.ones((), device=DEV).expand(rows.shape) if expanded
+                                     else torch.ones_like(rows), retain_graph=True)
+        return (*direct, *torch.autograd.grad((h, n), (x, w, gain), (d, d)))
+
+    assert all(torch.equal(a, b) for a, b in zip(leaves(True), leaves(False)))
+    alive = (idx >= 0).sum(1, keepdim=True).float().expand(T, H)
+    assert torch.equal(leaves(True)[0], alive)               # small integers: exact
+
+
+def test_two_graphs_replayed_in_turn():
+    """Each graph keeps its own index, workspaces and results while the other is replayed and eager calls run between."""
+    import terrace.ops as tops
+    announce("two graphs")
+    E, H = 16, 264
+    sets = []
+    for i, T in enumerate((900, 1500)):                      # the sorting path
+        x = torch.randn((T, H), generator=gen(50 + i), device=DEV).bfloat16()
+        idx = routing(T, E, 4, 60 + i, 0.1)
+        w = torch.rand((T, 4), generator=gen(70 + i), device=DEV).bfloat16()
+        sets.append((x, idx, w))
+
+    def step(x, idx, w):
+        rows, plan = tops.expert_sort(x, idx, E)
+        y = tops.expert_unsort(rows, w, plan)
+        return (rows, plan.offsets, *tops.block_norm(y, x, None, None, torch.ones((H,), dtype=x.dtype, device=DEV)))
+
+    graphs = []
+    for s in sets:
+        step(*s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*s)
+        graphs.append((graph, out))
+    for rep in range(3):
+        announce("two graphs", rep)
+        for i, (x, idx, _) in enumerate(sets):
+            x.copy_(torch.randn(x.shape, generator=gen(80 + 2 * rep + i), device=DEV).bfloat16())
+            idx.copy_(routing(x.shape[0], E, 4, 90 + 2 * rep + i, 0.1))
+        for graph, _ in graphs:
+            graph.replay()
+        want = [step(*s) for s in sets]
+        torch.cuda.synchronize()
+        for (_, out), eager in zip(graphs, want):
+            assert all(torch.equal(a, b) for a, b in zip(out, eager))
