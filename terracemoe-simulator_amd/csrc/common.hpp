@@ -64,6 +64,7 @@ __device__ __forceinline__ int wave_inclusive_scan(int v) {
 }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 template <typename V>

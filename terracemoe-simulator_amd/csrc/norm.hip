@@ -252,8 +252,8 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_kernel(NormArgs a, vo
 }
 
 // The gradient: 16384 rows of 7168 bf16, 1.41 GB, in 279 us, 5.0 TB/s.  By counters vector instructions fill
-// 55 % of the cycles and LDS bank conflicts 28 %, and the 14 waves of a row, alone on their CU, wait for each other once a
-// row.  512 workgroups took 385 us where 256 took 374-379.
+// 54 % of the cycles; the 14 waves of a row, alone on their CU, wait for each other once a row, which is likely the rest but
+// was not measured apart.  512 workgroups took 385 us where 256 took 374-379.
 // A workgroup walks the rows blockIdx.x * groups + group + i * gridDim.x * groups.  The next row is fetched
 // before the present one is reduced: the workgroup fills a CU, and without that nothing would be in flight while its
 // waves meet.  The vectors over the channels wait in LDS.  The sums over the rows stay in registers over the walk, two of
@@ -271,7 +271,8 @@ struct NormGrad {
 
 // A vector over the channels lies in LDS as two halves, the first and the last four of every piece of eight: neighbouring
 // lanes then read neighbouring 16 bytes.  (Pieces of 32 bytes back to back cost a bank conflict on every read: 1.5e8
-// cycles over the card in a gradient of 16384 rows of 7168, two thirds of its time on every CU.)
+// cycles over the card in a gradient of 16384 rows of 7168.  The halves read float by float still cost 4.4e7; as whole
+// 16 bytes 1e5, at the same time within the noise, 278-284 us and 280-281.)
 __device__ __forceinline__ int lds_slot(int c, int padded) { return (c & 4 ? padded / 2 : 0) + c / 8 * 4 + c % 4; }
 
 template <int E>
@@ -283,7 +284,11 @@ __device__ __forceinline__ void take_channels(bool given, const float *lds, int 
         for (int j = 0; j < 8; ++j) f[i * 8 + j] = fill;
         if (given && c < padded) {                           // whole pieces: the LDS rows are padded to them
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[i * 8 + j] = lds[lds_slot(c, padded) + j / 4 * (padded / 2) + j % 4];
+            for (int j = 0; j < 2; ++j) {
+                const f32x4 v = *(const f32x4 *)(lds + lds_slot(c, padded) + j * (padded / 2));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[i * 8 + j * 4 + k] = v[k];
+            }
         }
     }
 }
@@ -291,7 +296,7 @@ __device__ __forceinline__ void take_channels(bool given, const float *lds, int 
 template <int TY, int TR, bool ALIGNED, int E, bool WIDE>
 __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs a, NormGrad d) {
     __shared__ float part[2][kNormWaves * 3];
-    extern __shared__ float vectors[];                       // [2][H up to a piece]: w_post * gate, w_pre
+    extern __shared__ __align__(16) float vectors[];         // [2][H up to a piece]: w_post * gate, w_pre
     const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / a.tpr);          // whole waves per row
     const int at = (int)threadIdx.x - group * a.tpr;
     const float inv_h = 1.0f / (float)a.H;
