@@ -11,8 +11,11 @@
 // The two means need three sums that do not wait for each other -- sum(t v), sum((dh + inv2 t) q), sum(v q) -- because
 // sum(dH q) = sum((dh + inv2 t) q) - inv2 * mean(t v) * sum(v q), so a row costs one reduction.
 //
+// Without a gradient of n (or without w_pre) t is not there: dH = dh, and neither h nor v is made.
+//
 // All arithmetic is fp32; every output is rounded once.  n comes from the unrounded h, and the gradient recomputes h
-// from y and the residual (which it reads instead of h: the same bytes), so no stored rounding enters it.
+// from y and the residual, so no stored rounding enters it.  With a post norm or a gate y is needed anyway and the
+// residual is read in the place of h, the same bytes; with neither, y and the residual are read where h alone would do.
 #include "common.hpp"
 
 namespace terrace {
@@ -261,6 +264,9 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_kernel(NormArgs a, vo
 // row partial[2][gridDim.x][H] of sum(factor dH u) and sum(dn v), and norm_reduce_kernel adds those up in order.
 // WIDE (16 elements a lane): the sums are kept in the partial row itself, which the lane that owns the channel reads and
 // writes row by row, the vectors come from cache, and no row is fetched ahead.
+//
+// DN: there is a gradient of n.  Without one the residual is not read and nothing of h is formed, so an infinity or a NaN
+// in it (or in y, without a post norm) reaches no sum that it is not a term of.
 struct NormGrad {
     const void *dh, *dn;                                     // either may be NULL
     const float *stats;
@@ -293,7 +299,7 @@ __device__ __forceinline__ void take_channels(bool given, const float *lds, int 
     }
 }
 
-template <int TY, int TR, bool ALIGNED, int E, bool WIDE>
+template <int TY, int TR, bool ALIGNED, int E, bool WIDE, bool DN>
 __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs a, NormGrad d) {
     __shared__ float part[2][kNormWaves * 3];
     extern __shared__ __align__(16) float vectors[];         // [2][H up to a piece]: w_post * gate, w_pre
@@ -303,7 +309,8 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
     const int64_t stride = (int64_t)gridDim.x * a.groups;
     const void *channel_gate = a.gate_kind == TERRACE_GATE_CHANNEL ? a.gate : nullptr;
     const int padded = (int)((a.H + 7) / 8 * 8);
-    const bool has_b = a.w_post || channel_gate;
+    const bool has_b = a.w_post || channel_gate, need_y = a.y && (DN || a.w_post || a.gate);
+    const bool need_dot = a.w_post || d.d_token;
     float *lds_b = vectors, *lds_pre = vectors + padded;
     if constexpr (!WIDE) {
         for (int c = threadIdx.x; c < padded; c += blockDim.x) {
@@ -312,7 +319,7 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
             if (a.w_post && in) b *= load_scalar(a.w_post, a.post_dtype, c);
             if (channel_gate && in) b *= load_scalar(channel_gate, a.gate_dtype, c);
             if (has_b) lds_b[lds_slot(c, padded)] = b;
-            if (a.w_pre) lds_pre[lds_slot(c, padded)] = in ? load_scalar(a.w_pre, a.pre_dtype, c) : 0.0f;
+            if (DN) lds_pre[lds_slot(c, padded)] = in ? load_scalar(a.w_pre, a.pre_dtype, c) : 0.0f;
         }
         __syncthreads();
     }
@@ -322,12 +329,12 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
             float g[E];
             load_channels<ALIGNED, E>(a.w_post, a.post_dtype, a.H, at, a.tpr, 1.0f, b);
             load_channels<ALIGNED, E>(channel_gate, a.gate_dtype, a.H, at, a.tpr, 1.0f, g);
-            load_channels<ALIGNED, E>(a.w_pre, a.pre_dtype, a.H, at, a.tpr, 0.0f, wn);
+            if constexpr (DN) load_channels<ALIGNED, E>(a.w_pre, a.pre_dtype, a.H, at, a.tpr, 0.0f, wn);
 #pragma unroll
             for (int e = 0; e < E; ++e) b[e] *= g[e];
         } else {
             take_channels<E>(has_b, lds_b, padded, at, a.tpr, 1.0f, b);
-            take_channels<E>(a.w_pre != nullptr, lds_pre, padded, at, a.tpr, 0.0f, wn);
+            if constexpr (DN) take_channels<E>(true, lds_pre, padded, at, a.tpr, 0.0f, wn);
         }
     };
     float sum[2][WIDE ? 1 : E];
@@ -344,12 +351,12 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
         x.y.clear(), x.r.clear(), x.dh.clear(), x.dn.clear();
         x.inv1 = x.inv2 = x.token = 1.0f;
         if (row >= a.T) return;
-        if (a.y) x.y.load(a.y, row, a.H, at, a.tpr);
-        x.r.load(a.residual, row, a.H, at, a.tpr);
+        if (need_y) x.y.load(a.y, row, a.H, at, a.tpr);
+        if constexpr (DN) x.r.load(a.residual, row, a.H, at, a.tpr);
         if (d.dh) x.dh.load(d.dh, row, a.H, at, a.tpr);
-        if (d.dn) x.dn.load(d.dn, row, a.H, at, a.tpr);
+        if constexpr (DN) x.dn.load(d.dn, row, a.H, at, a.tpr);
         x.inv1 = d.stats[2 * row];
-        x.inv2 = d.stats[2 * row + 1];
+        if constexpr (DN) x.inv2 = d.stats[2 * row + 1];
         if (a.gate_kind == TERRACE_GATE_TOKEN) x.token = load_scalar(a.gate, a.gate_dtype, row);
     };
     const int64_t first = (int64_t)blockIdx.x * a.groups;
@@ -360,38 +367,51 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_grad_kernel(NormArgs 
         const int64_t row = base + group;
         const bool mine = row < a.T;
         if constexpr (!WIDE) fetch(row + stride, next);
-        float s[3] = {0.0f, 0.0f, 0.0f};
         const float factor = a.scale * cur.token;            // scale, and the token's gate where there is one
         float b[E], wn[E];
         take(b, wn);
+        float mean_tv = 0.0f, dot;                           // dot: sum of dH * gate per channel * p
+        if constexpr (DN) {
+            float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float u = cur.y.get(e) * cur.inv1, q = u * b[e];
-            const float h = __fmaf_rn(factor, q, cur.r.get(e)), v = h * cur.inv2, t = cur.dn.get(e) * wn[e];
-            s[0] = __fmaf_rn(t, v, s[0]);
-            s[1] = __fmaf_rn(__fmaf_rn(cur.inv2, t, cur.dh.get(e)), q, s[1]);
-            s[2] = __fmaf_rn(v, q, s[2]);
+            for (int e = 0; e < E; ++e) {
+                const float u = cur.y.get(e) * cur.inv1, q = u * b[e];
+                const float h = __fmaf_rn(factor, q, cur.r.get(e)), v = h * cur.inv2, t = cur.dn.get(e) * wn[e];
+                s[0] = __fmaf_rn(t, v, s[0]);
+                s[1] = __fmaf_rn(__fmaf_rn(cur.inv2, t, cur.dh.get(e)), q, s[1]);
+                s[2] = __fmaf_rn(v, q, s[2]);
+            }
+            row_sum<3>(s, part[turn], a.tpr);
+            mean_tv = s[0] * inv_h;
+            dot = __fmaf_rn(-cur.inv2 * mean_tv, s[2], s[1]);
+        } else {
+            dot = 0.0f;
+            if (need_dot) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) dot = __fmaf_rn(cur.dh.get(e), cur.y.get(e) * cur.inv1 * b[e], dot);
+                row_sum<1>(&dot, part[turn], a.tpr);
+            }
         }
-        row_sum<3>(s, part[turn], a.tpr);
         turn ^= 1;
-        const float mean_tv = s[0] * inv_h;
-        const float dot = __fmaf_rn(-cur.inv2 * mean_tv, s[2], s[1]);         // sum of dH * gate per channel * p
         const float mean_u = factor * dot * inv_h;
         take(b, wn);
         float o1[E], o2[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float u = cur.y.get(e) * cur.inv1;
-            const float h = __fmaf_rn(factor, u * b[e], cur.r.get(e)), v = h * cur.inv2;
-            const float dn = cur.dn.get(e);
-            const float dH = __fmaf_rn(cur.inv2, __fmaf_rn(-v, mean_tv, dn * wn[e]), cur.dh.get(e));
+            float v = 0.0f, dn = 0.0f, dH = cur.dh.get(e);
+            if constexpr (DN) {
+                v = __fmaf_rn(factor, u * b[e], cur.r.get(e)) * cur.inv2;
+                dn = cur.dn.get(e);
+                dH = __fmaf_rn(cur.inv2, __fmaf_rn(-v, mean_tv, dn * wn[e]), dH);
+            }
             const float z = factor * dH;
             o1[e] = dH;
             o2[e] = z * b[e];
             if (a.w_post) o2[e] = cur.inv1 * __fmaf_rn(-u, mean_u, o2[e]);
             if constexpr (!WIDE) {
                 sum[0][e] = __fmaf_rn(z, u, sum[0][e]);
-                sum[1][e] = __fmaf_rn(dn, v, sum[1][e]);
+                if constexpr (DN) sum[1][e] = __fmaf_rn(dn, v, sum[1][e]);
             } else if (mine) {                               // one group: this lane alone touches the channel's cells
                 const int64_t c = ((int64_t)at + (int64_t)(e / 8) * a.tpr) * 8 + e % 8;
                 if (c < a.H) {
@@ -595,13 +615,17 @@ int run_block_norm_grad(const void *y, int y_dtype, const void *residual, int r_
                          want_v};
         const unsigned threads = (unsigned)(a.tpr * a.groups);
         const size_t lds = form.per == 16 ? 0 : (size_t)(2 * ((H + 7) / 8 * 8)) * sizeof(float);
-#define TERRACE_NORM(Y, R)                                                                                              \
-    if (form.aligned && form.per == 8) block_norm_grad_kernel<Y, R, true, 8, false><<<grid, threads, lds, s>>>(a, d);    \
-    else if (form.aligned) block_norm_grad_kernel<Y, R, true, 16, true><<<grid, threads, lds, s>>>(a, d);                \
-    else if (form.per == 8) block_norm_grad_kernel<Y, R, false, 8, false><<<grid, threads, lds, s>>>(a, d);              \
-    else block_norm_grad_kernel<Y, R, false, 16, true><<<grid, threads, lds, s>>>(a, d)
+#define TERRACE_NORM_FORM(Y, R, A, E, WIDE)                                                                     \
+    if (dn) block_norm_grad_kernel<Y, R, A, E, WIDE, true><<<grid, threads, lds, s>>>(a, d);                   \
+    else block_norm_grad_kernel<Y, R, A, E, WIDE, false><<<grid, threads, lds, s>>>(a, d)
+#define TERRACE_NORM(Y, R)                                                               \
+    if (form.aligned && form.per == 8) { TERRACE_NORM_FORM(Y, R, true, 8, false); }      \
+    else if (form.aligned) { TERRACE_NORM_FORM(Y, R, true, 16, true); }                  \
+    else if (form.per == 8) { TERRACE_NORM_FORM(Y, R, false, 8, false); }                \
+    else { TERRACE_NORM_FORM(Y, R, false, 16, true); }
         TERRACE_NORM_TYPES(TERRACE_NORM)
 #undef TERRACE_NORM
+#undef TERRACE_NORM_FORM
     }
     if (sums)
         norm_reduce_kernel<<<dim3((unsigned)((H + kWave - 1) / kWave), 2), 1024, 0, s>>>((const float *)ws, (int)grid, a, red);

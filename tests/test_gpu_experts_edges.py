@@ -1,0 +1,81 @@
+"""The operators around the experts at the edges of what they take: values that are not finite or very large, derivatives
+they do not have, handles that do not fit, and sizes on both sides of each choice of kernel."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_experts import announce, near, norm_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def same(a, b):
+    """Equal bits, NaN included."""
+    return torch.equal(a.detach().view(torch.uint8), b.detach().view(torch.uint8))
+
+
+# ---- block_norm without a gradient of n ---------------------------------------------------------------------------
+@pytest.mark.parametrize("T,H", [(70, 264), (530, 1001), (40, 9000), (300, 8193)])
+@pytest.mark.parametrize("dtype,residual", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("post,gate", [(False, None), (False, "channel"), (False, "token"), (True, "channel"), (True, "token")])
+@pytest.mark.parametrize("pre", [False, True])
+def test_block_norm_gradient_of_h_alone_keeps_what_is_not_finite_in_its_place(T, H, dtype, residual, post, gate, pre):
+    """Only h is differentiated: its gradient does not depend on the residual, and without a post norm on y only through
+    the gate's own gradient, so an infinity or a NaN there changes no other bit."""
+    import terrace.ops as tops
+    announce("block_norm not finite", T, H, dtype, residual, post, gate, pre)
+    y, r, wp, gt, wn, dh, _ = norm_inputs(T, H, dtype, residual, True, post, gate, pre, T + H)
+
+    def grads(y, r):
+        leaves = {n: t.detach().clone().requires_grad_(True) for n, t in
+                  (("y", y), ("residual", r), ("post", wp), ("gate", gt), ("pre", wn)) if t is not None}
+        h, _ = tops.block_norm(leaves["y"], leaves["residual"], leaves.get("post"), leaves.get("gate"), leaves.get("pre"),
+                               scale=0.75)
+        return dict(zip(leaves, torch.autograd.grad(h, list(leaves.values()), dh, allow_unused=True)))
+
+    clean = grads(y, r)
+    assert torch.equal(clean["residual"], dh)
+    bad = r.clone()
+    bad[3, 5], bad[7, H - 1], bad[T - 1, 0] = float("inf"), float("nan"), float("-inf")
+    for name, g in grads(y, bad).items():
+        if name == "pre":
+            assert g is None or not bool(g.ne(0).any())
+        else:
+            assert same(g, clean[name]), name
+    if post:
+        return
+    bad = y.clone()
+    bad[11, 13], bad[20, H - 2] = float("inf"), float("nan")
+    got = grads(bad, r)
+    assert same(got["residual"], clean["residual"]) and same(got["y"], clean["y"])
+    if gate == "channel":
+        off = ~got["gate"].isfinite()
+        assert off.nonzero()[:, 0].tolist() == [13, H - 2]
+        assert same(got["gate"][~off], clean["gate"][~off])
+    elif gate == "token":
+        off = ~got["gate"][:, 0].isfinite()
+        assert off.nonzero()[:, 0].tolist() == [11, 20]
+        assert same(got["gate"][~off], clean["gate"][~off])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("gate", ["token", "channel"])
+def test_block_norm_gradient_of_h_alone_on_very_large_values(dtype, gate):
+    """|y| about 2^66 without a norm: the products with the gradients stay in range, the squares would not."""
+    import terrace.ops as tops
+    announce("block_norm large", dtype, gate)
+    T, H = 60, 520
+    y, r, _, gt, _, dh, _ = norm_inputs(T, H, dtype, dtype, True, False, gate, False, 5)
+    y, r = y * 2.0 ** 65, r * 2.0 ** 66
+    leaves = [t.requires_grad_(True) for t in (y, r, gt)]
+    h, n = tops.block_norm(y, r, None, gt, None)
+    dy, dr, dg = torch.autograd.grad(h, leaves, dh)
+    assert n is None and torch.equal(dr, dh)
+    gd, dhd, yd = gt.detach().double(), dh.double(), y.detach().double()
+    near(dy, gd * dhd, (gd * dhd).abs(), 2, "d_y")
+    terms = yd * dhd
+    if gate == "token":
+        near(dg, terms.sum(1, keepdim=True), terms.abs().sum(1, keepdim=True), H / 64 + 40, "d_gate")
+    else:
+        near(dg, terms.sum(0), terms.abs().sum(0), T + 40, "d_gate")
