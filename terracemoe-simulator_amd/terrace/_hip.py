@@ -12,6 +12,7 @@ import os
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 ENV_LIB = "TERRACE_OPS_LIB"
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -196,6 +197,17 @@ def need_device(*tensors):
         if t is not None and not t.is_cuda:
             raise RuntimeError("terrace (MI355X build): tensors must live on a ROCm device; this build has no "
                                "CPU path")
+
+
+def refuse_tangents(*tensors):
+    """Raises when one of the tensors (None: absent) carries a forward-mode tangent, which a library call would drop
+    without a word: nothing here implements forward-mode derivatives.  A level is open only inside ``dual_level``, and
+    ``inference_mode`` switches tangents off as it does for torch's own operators."""
+    if _forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("terrace: forward-mode derivatives are not implemented (an argument carries a tangent)")
 
 
 def ptr(t):

@@ -4,7 +4,8 @@
 
 They have no counterpart in the reference, which leaves them to the layer around it.  As everywhere in ``terrace.ops``
 the kernels of the library are the only implementation: a tensor that is not on a ROCm device raises, and every call
-enqueues on the current stream of its tensors' device.
+enqueues on the current stream of its tensors' device.  Gradients are those of reverse mode; a tensor with a forward-mode
+tangent raises.
 """
 from __future__ import annotations
 
@@ -22,8 +23,10 @@ _CURRENT = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _ready(*tensors) -> int:
-    """The library is loaded and the tensors (None: absent) share one ROCm device, whose index is returned."""
+    """The library is loaded and the tensors (None: absent) share one ROCm device, whose index is returned; none carries
+    a forward-mode tangent."""
     _ops._require()
+    _hip.refuse_tangents(*tensors)
     index = -1
     for t in tensors:
         if t is None:
@@ -157,6 +160,7 @@ class _ExpertSortFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
+        _hip.refuse_tangents(g)
         (planes,) = ctx.saved_tensors
         T, k, dtype = ctx.geom
         return _combine(g.get_device(), g.contiguous(), planes.data_ptr(), None, T, k, dtype), None, None, None, None, None
@@ -204,6 +208,7 @@ class _ExpertUnsortFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _hip.refuse_tangents(dy)
         rows, weights, planes = ctx.saved_tensors
         T, k, n = ctx.geom
         dy = dy.contiguous()
@@ -361,6 +366,7 @@ class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dn):
+        _hip.refuse_tangents(dh, dn)
         y, residual, post_weight, gate, pre_weight, stats = ctx.saved_tensors
         kind, scale, eps = ctx.norm
         T, H = residual.shape

@@ -122,3 +122,25 @@ def test_the_experts_of_one_layer_must_fit_each_other():
                  (w(4, 64, 128), w(4, 128, 32, torch.float16))):
         with pytest.raises(RuntimeError, match="cannot feed"):
             w4_experts(a, b)
+
+
+def test_a_forward_mode_tangent_is_refused():
+    import torch.autograd.forward_ad as fwAD
+    import terrace.ops as tops
+    x, idx = torch.zeros(4, 32), torch.zeros(4, 2, dtype=torch.int64)
+    plan = tops.ExpertPlan(torch.zeros(8 + 8 + 3, dtype=torch.int64), 4, 2, 4)
+    weights = tops.W4Weights(torch.zeros(1, dtype=torch.uint8), None, None, 1, 32, 32, 32, torch.float32)
+    with fwAD.dual_level():
+        d = fwAD.make_dual(x, torch.ones_like(x))
+        rows, w = (fwAD.make_dual(t, torch.ones_like(t)) for t in (torch.zeros(8, 32), torch.zeros(4, 2)))
+        calls = [lambda: tops.expert_sort(d, idx, 4), lambda: tops.expert_unsort(rows, None, plan),
+                 lambda: tops.expert_unsort(torch.zeros(8, 32), w, plan), lambda: tops.block_norm(d, x),
+                 lambda: tops.block_norm(x, d), lambda: tops.block_norm(x, x, d[0]), lambda: tops.block_norm(x, x, None, d[0]),
+                 lambda: tops.block_norm(None, x, pre_weight=d[0]), lambda: tops.expert_linear_w4(d, None, weights)]
+        for f in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f()
+        with pytest.raises(RuntimeError, match="ROCm device"):          # a level alone is no tangent
+            tops.block_norm(x, x)
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="ROCm device"):
+            tops.block_norm(d, x)

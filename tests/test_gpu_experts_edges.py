@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_experts import announce, near, norm_inputs
+from test_gpu_experts import DEV, announce, gen, near, norm_inputs, routing
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,30 @@ def test_block_norm_gradient_of_h_alone_on_very_large_values(dtype, gate):
         near(dg, terms.sum(1, keepdim=True), terms.abs().sum(1, keepdim=True), H / 64 + 40, "d_gate")
     else:
         near(dg, terms.sum(0), terms.abs().sum(0), T + 40, "d_gate")
+
+
+# ---- forward mode -------------------------------------------------------------------------------------------------
+def test_no_operator_drops_a_forward_mode_tangent():
+    """Neither in the forward call nor in a backward pass whose incoming gradient carries one."""
+    import torch.autograd.forward_ad as fwAD
+    import terrace.ops as tops
+    announce("forward mode")
+    T, E, k, H = 20, 4, 2, 64
+    x, idx = torch.randn((T, H), generator=gen(1), device=DEV), routing(T, E, k, 2)
+    rows, plan = tops.expert_sort(x, idx, E)
+    w = torch.rand((T, k), generator=gen(3), device=DEV)
+    leaf = x.clone().requires_grad_(True)
+    results = [tops.expert_sort(leaf, idx, E)[0], tops.expert_unsort(rows.clone().requires_grad_(True), w, plan),
+               tops.block_norm(leaf, x)[0]]
+    with fwAD.dual_level():
+        dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))
+        for f in (lambda: tops.expert_sort(dual(x), idx, E), lambda: tops.expert_unsort(dual(rows), w, plan),
+                  lambda: tops.expert_unsort(rows, dual(w), plan), lambda: tops.block_norm(dual(x), x),
+                  lambda: tops.block_norm(x, x, None, None, dual(x[0]))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f()
+        for out in results:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                out.backward(dual(torch.ones_like(out)))
+        again, _ = tops.expert_sort(x, idx, E)               # a level alone changes nothing
+    assert torch.equal(again, rows)
