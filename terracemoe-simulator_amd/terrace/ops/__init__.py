@@ -1137,6 +1137,7 @@ class TerraceK1ArrivalFn(torch.autograd.Function):
 def k1_arrival(rx, rslot, rgate, quota: int, epr: int, rpn: int, my_local: int = 0):
     """Arrival-side fused chain: (send_buf, gate_pairs, r_idx, slot_idx, i_send)."""
     _require()
+    _hip.refuse_tangents(rx, rgate)
     if rx.requires_grad or rgate.requires_grad:
         return TerraceK1ArrivalFn.apply(rx, rslot, rgate, quota, epr, rpn, my_local)
     return k1_arrival_raw(rx, rslot, rgate, quota, epr, rpn, my_local)
@@ -1228,6 +1229,7 @@ def k2_pack(hidden, expert_idx, gates, world: int, n_experts: int, rpn: int, gro
     """Send-side fused chain: (payload, mask, gate_rows, u_src, node_counts).  ``payload`` and ``gate_rows``
     carry gradients to ``hidden`` and ``gates``; a malformed routing raises ValueError on the guard's cadence."""
     _require()
+    _hip.refuse_tangents(hidden, gates)
     if torch.is_grad_enabled() and (hidden.requires_grad or gates.requires_grad):
         return TerraceK2PackFn.apply(hidden, expert_idx, gates, world, n_experts, rpn, groups_m)
     out, ex = k2_pack_raw(hidden, expert_idx, gates, world, n_experts, rpn, groups_m, extras=True)

@@ -19,6 +19,7 @@ def k2_pack_ref(hidden: torch.Tensor, expert_idx: torch.Tensor, gates: torch.Ten
     """(payload [T*M, H], mask [T*M, q] int64 ascending slot ids, gate_rows [T*M, q], u_src [T*M] int64,
     node_counts [n_nodes] int64); ``payload`` and ``gate_rows`` carry gradients."""
     _require()
+    _hip.refuse_tangents(hidden, gates)
     _hip.need_device(hidden, expert_idx, gates)
     _check_k2(hidden, expert_idx, gates, world, n_experts, rpn, groups_m)
     slots = (n_experts // world) * rpn

@@ -110,6 +110,7 @@ def ta2a_permute(hidden_states, probs, routing_map, *, world, rank, rpn, n_exper
     """Dispatch half: (permuted [P,H], tokens_per_expert, permuted_probs [P], state)."""
     _loopback_only(intra_group, inter_group)
     _ops._require()
+    _hip.refuse_tangents(hidden_states, probs)
     _hip.need_device(hidden_states, probs, routing_map)
     epr = n_experts // world
     slots = epr * rpn
@@ -211,6 +212,7 @@ def ta2a_unpermute(expert_out, st: TA2AState, out_like):
     reference: a send row sums the outputs of its (row, slot) pairs in arrival order, a token sums
     its rows in ascending row order; each level accumulates in fp32 and rounds once to the
     tensor dtype."""
+    _hip.refuse_tangents(expert_out)
     _hip.need_device(expert_out)
     if torch.is_grad_enabled() and expert_out.requires_grad:
         return _UnpermuteFn.apply(expert_out, st.red_table, st.tok_table, st.where, out_like.dtype)

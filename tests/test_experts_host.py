@@ -144,3 +144,22 @@ def test_a_forward_mode_tangent_is_refused():
             tops.block_norm(x, x)
         with torch.inference_mode(), pytest.raises(RuntimeError, match="ROCm device"):
             tops.block_norm(d, x)
+
+
+def test_a_forward_mode_tangent_is_refused_by_the_operators_of_the_path_that_carry_gradients():
+    import torch.autograd.forward_ad as fwAD
+    import terrace.ops as tops
+    from terrace.ops.k2_ref import k2_pack_ref
+    from terrace.ta2a_dispatch import ta2a_permute, ta2a_unpermute
+    x, idx, gates, probs = torch.zeros(4, 32), torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2), torch.zeros(4, 8)
+    with fwAD.dual_level():
+        dx, dg = (fwAD.make_dual(t, torch.ones_like(t)) for t in (x, gates))
+        dp = fwAD.make_dual(probs, torch.ones_like(probs))
+        geometry = dict(world=4, rank=0, rpn=2, n_experts=8)
+        calls = [lambda: tops.k1_arrival(dx, idx, gates, 2, 2, 2), lambda: tops.k1_arrival(x, idx, dg, 2, 2, 2),
+                 lambda: tops.k2_pack(dx, idx, gates, 4, 8, 2, 2), lambda: tops.k2_pack(x, idx, dg, 4, 8, 2, 2),
+                 lambda: k2_pack_ref(dx, idx, gates, 4, 8, 2, 2), lambda: ta2a_permute(dx, probs, probs > 0, **geometry),
+                 lambda: ta2a_permute(x, dp, probs > 0, **geometry), lambda: ta2a_unpermute(dx, None, x)]
+        for f in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f()
