@@ -21,7 +21,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // f16: bits 6-9): one turn and one and-or for two codes.  The constant is taken out again group by group,
 //   sum_k (c - z) x = sum_k (16 + c) x - (16 + z) * sum_k x,
 // the second sum by matrix instructions too (w4_use).  Everything is added in fp32, so the constant costs 2-3 bits of
-// 24, not of the inputs' 8 or 11.
+// 24, not of the inputs' 8 or 11.  An infinite x, or a bf16 x whose multiples pass 2^128, makes both sums infinite where
+// their difference need not be: a result that is not finite is taken again from the definition (w4_plain).
 template <int DT>
 struct W4Type;
 template <>
@@ -382,6 +383,40 @@ __device__ __forceinline__ void w4_use(W4Block<T, 4 / GS, ZEROS> &k, X x, f32x4 
     }
 }
 
+__device__ __forceinline__ bool w4_finite(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
+
+// One result from the definition, sum_k (scale * (code - zero)) * x[k] over k in order, by one lane: an infinite x gives
+// an infinity, or NaN where its weight is 0, and a finite sum is found although (16 + code) x left the range.  Reached by
+// results that are not finite only; what waits in it is one lane's chain of loads.  One token through the gate and up
+// projections of 8 experts (4096 x 7168): 27 us, 420 with one infinite row, 750 with all eight; 2048 rows over 64 experts
+// of 4096 x 4096: 155 us, 1.0 ms with one, 13.5 ms with every row infinite.
+template <int DT, int GS, bool ZEROS>
+__device__ __forceinline__ float w4_plain(const W4Args &a, const W4Expert &e, int col, const uint8_t *row) {
+    constexpr int kGpb = 4 / GS;
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int k = 0; k < (int)a.sh.K; k += 8) {               // one dword of codes; K is a multiple of 32
+        const int block = k / kBlockK, step = k / 32 % 4;
+        const W4Column c = w4_column(a, col, k / 8 % 4, kGpb);
+        const uint32_t w = *(const uint32_t *)(e.codes + (int64_t)block * 1024 + c.codes + 4 * step);
+        const uint32_t codes = __builtin_amdgcn_alignbit(w, w, W4Type<DT>::kShift);          // as before the turn of the packing
+        const int64_t group = (int64_t)block * (kGpb * kTileN) + c.groups + step / GS;
+        const uint32_t s = ((const uint16_t *)e.scales)[group];
+        float scale;
+        if constexpr (DT == TERRACE_BF16) scale = bf16_bits_to_f32(s);
+        else scale = __half2float(__ushort_as_half((unsigned short)s));
+        const int zero = ZEROS ? (int)e.zeros[group] : 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int code = (int)(codes >> (4 * (i / 2) + 16 * (i & 1))) & 15;
+            float x;
+            load_floats<DT, 1>(row, k + i, &x);
+            sum = __fmaf_rn(scale * (float)(code - zero), x, sum);
+        }
+    }
+    return sum;
+}
+
 __device__ __forceinline__ float w4_swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
 
 // Few rows: tiles of 16.  One token through the gate and up projections of 8 experts (121 MB) 25 us, 4.8 TB/s; 512 rows
@@ -457,9 +492,11 @@ __global__ __launch_bounds__(kMaxSplit * kWave) void w4_few_kernel(W4Args a) {
         }
         use(f);
     }
+    uint32_t again = 0;                                      // rows of this lane's quarter with a sum that is not finite
     auto store = [&](int i, float v0, float v1) {            // row i of this lane's quarter
         const int row = 4 * q + i;
         if (row >= rt.rows) return;
+        if (!w4_finite(v0) || !w4_finite(v1)) again |= 1u << i;
         uint16_t *o = (uint16_t *)a.out + (int64_t)(rt.first + row) * a.out_cols;
         if (a.swiglu) {
             if (col0 < a.out_cols) o[col0] = (uint16_t)to_bits16<DT>(w4_swiglu(v0, v1));
@@ -471,21 +508,33 @@ __global__ __launch_bounds__(kMaxSplit * kWave) void w4_few_kernel(W4Args a) {
     if (a.split == 1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) store(i, total[0][0][i], total[0][1][i]);
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        lds[w][i][lane] = total[0][0][i];
-        lds[w][4 + i][lane] = total[0][1][i];
-    }
-    __syncthreads();
-    for (int i = part; i < 4; i += a.split) {
-        float v0 = 0.0f, v1 = 0.0f;
-        for (int y = w - part; y < w - part + a.split; ++y) {
-            v0 += lds[y][i][lane];
-            v1 += lds[y][4 + i][lane];
+        for (int i = 0; i < 4; ++i) {
+            lds[w][i][lane] = total[0][0][i];
+            lds[w][4 + i][lane] = total[0][1][i];
         }
-        store(i, v0, v1);
+        __syncthreads();
+        for (int i = part; i < 4; i += a.split) {
+            float v0 = 0.0f, v1 = 0.0f;
+            for (int y = w - part; y < w - part + a.split; ++y) {
+                v0 += lds[y][i][lane];
+                v1 += lds[y][4 + i][lane];
+            }
+            store(i, v0, v1);
+        }
+    }
+    for (uint32_t left = again; left; left &= left - 1) {
+        const int i = __builtin_ctz(left);
+        const uint8_t *row = xt + (int64_t)(4 * q + i) * a.sh.K * 2;
+        float v[2];
+#pragma unroll 1
+        for (int j = 0; j < 2; ++j) {
+            const float r = w4_plain<DT, GS, ZEROS>(a, we, j ? col1 : col0, row);
+            v[0] = j ? v[0] : r;
+            v[1] = r;
+        }
+        store(i, v[0], v[1]);
     }
 }
 
@@ -513,13 +562,11 @@ __global__ __launch_bounds__(4 * kWave, 2) void w4_many_kernel(W4Args a) {
     }
     const int c16 = lane & 15, q = lane >> 4;
     const W4Expert we = w4_expert(a, rt.expert, 4 / GS);
-    int at[T];
+    // swiglu: tiles 0 and 2 of the first half, 1 and 3 their partners
+    auto column = [&](int t) { return lo + w * width + (a.swiglu ? (t >> 1) * 16 + (t & 1) * a.out_cols : t * 16); };
     W4Column col[T];
 #pragma unroll
-    for (int t = 0; t < T; ++t) {                            // swiglu: tiles 0 and 2 of the first half, 1 and 3 their partners
-        at[t] = lo + w * width + c16 + (a.swiglu ? (t >> 1) * 16 + (t & 1) * a.out_cols : t * 16);
-        col[t] = w4_column(a, at[t], q, 4 / GS);
-    }
+    for (int t = 0; t < T; ++t) col[t] = w4_column(a, column(t) + c16, q, 4 / GS);
     // wave w brings step w of a block: rows past the tile's last repeat it (their results are dropped), and a step past K
     // reads what is there and is masked to zeros, so that every load of the loop is unconditional
     const bool short_k = a.full == 0 && w >= a.rest;
@@ -574,23 +621,47 @@ __global__ __launch_bounds__(4 * kWave, 2) void w4_many_kernel(W4Args a) {
         }
     }
     if (b < blocks) use(0);
+    // the results of a lane in pairs: tiles 2p and 2p + 1, with `swiglu` a gate and its partner; the lane's place is worked
+    // out again here, so that nothing of it is kept over the loop
+    int late = lane;
+    asm volatile("" : "+v"(late));
+    const int row0 = 4 * (late >> 4), col0 = late & 15;
+    uint32_t again = 0;                                      // pairs with a sum that is not finite
+    auto store = [&](int row, int c0, int c1, float v0, float v1) {
+        uint16_t *o = (uint16_t *)a.out + (int64_t)(rt.first + row) * a.out_cols;
+        if (a.swiglu) {
+            if (c0 < a.out_cols) o[c0] = (uint16_t)to_bits16<DT>(w4_swiglu(v0, v1));
+        } else {
+            if (c0 < a.out_cols) o[c0] = (uint16_t)to_bits16<DT>(v0);
+            if (c1 < a.out_cols) o[c1] = (uint16_t)to_bits16<DT>(v1);
+        }
+    };
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int row = 16 * m + 4 * q + i;
+            const int row = 16 * m + i + row0;
             if (row >= rt.rows) continue;
-            uint16_t *o = (uint16_t *)a.out + (int64_t)(rt.first + row) * a.out_cols;
-            if (a.swiglu) {
 #pragma unroll
-                for (int t = 0; t < T; t += 2)
-                    if (at[t] < a.out_cols) o[at[t]] = (uint16_t)to_bits16<DT>(w4_swiglu(total[m][t][i], total[m][t + 1][i]));
-            } else {
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-                    if (at[t] < a.out_cols) o[at[t]] = (uint16_t)to_bits16<DT>(total[m][t][i]);
+            for (int p = 0; p < T / 2; ++p) {
+                const float v0 = total[m][2 * p][i], v1 = total[m][2 * p + 1][i];
+                if (!w4_finite(v0) || !w4_finite(v1)) again |= 1u << ((m * 4 + i) * (T / 2) + p);
+                store(row, column(2 * p) + col0, column(2 * p + 1) + col0, v0, v1);
             }
         }
+    }
+    for (uint32_t left = again; left; left &= left - 1) {
+        const int bit = __builtin_ctz(left), row = bit / (T / 2) / 4 * 16 + bit / (T / 2) % 4 + row0, p = bit % (T / 2);
+        const int c0 = column(2 * p) + col0, c1 = column(2 * p + 1) + col0;
+        const uint8_t *x = xt + (int64_t)row * a.sh.K * 2;
+        float v[2];
+#pragma unroll 1
+        for (int j = 0; j < 2; ++j) {
+            const float r = w4_plain<DT, GS, ZEROS>(a, we, j ? c1 : c0, x);
+            v[0] = j ? v[0] : r;
+            v[1] = r;
+        }
+        store(row, c0, c1, v[0], v[1]);
     }
 }
 

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_experts import DEV, announce, gen, near, norm_inputs, routing
+from test_gpu_experts import DEV, DT, announce, gen, near, norm_inputs, routing, w4_case
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,51 @@ def test_no_operator_drops_a_forward_mode_tangent():
                 out.backward(dual(torch.ones_like(out)))
         again, _ = tops.expert_sort(x, idx, E)               # a level alone changes nothing
     assert torch.equal(again, rows)
+
+
+# ---- 4-bit products of rows that are not finite or very large ------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("E,N,K,group,zeros,swiglu,counts", [
+    (1, 40, 1024, 128, False, False, [1]), (1, 256, 96, 32, True, False, [5]), (2, 50, 192, 64, True, True, [16, 15]),
+    (3, 33, 288, 32, False, False, [0, 9, 4]), (4, 64, 2048, 128, False, True, [1, 0, 0, 6]),
+    (2, 11000, 160, 32, True, True, [130, 40]), (3, 20000, 128, 128, False, False, [20, 33, 1]),
+    (1, 16400, 96, 32, False, True, [250]), (2, 24010, 448, 64, True, False, [64, 64]),
+])
+def test_w4_products_of_rows_that_are_not_finite_or_very_large(E, N, K, group, zeros, swiglu, counts, dtype):
+    """An infinite input gives what the definition gives -- an infinity, or NaN where its weight is 0 -- a NaN gives NaN,
+    very large inputs a finite result where there is one, and the other rows keep their bits."""
+    import terrace.ops as tops
+    announce("w4 not finite", E, N, K, group, dtype, zeros, swiglu, counts)
+    codes, scales, z, weight, size = w4_case(E, N, K, group, dtype, zeros, N + K)
+    packed = tops.w4_pack(codes, scales, z)
+    P = sum(counts)
+    tokens = torch.tensor(counts, device=DEV)
+    clean = torch.randn((P, K), generator=gen(K), device=DEV).to(DT[dtype])
+    expert = [e for e, c in enumerate(counts) for _ in range(c)]
+    x = clean.clone()
+    bad = {0: [float("inf")], P - 1: [float("-inf"), float("inf")], P // 2: [float("nan")]}
+    for n, (row, values) in enumerate(bad.items()):
+        for i, v in enumerate(values):
+            x[row, (37 * n + 61 * i + K - 1) % K] = v
+    large = [r for r in (1, P - 2) if 0 <= r < P and r not in bad] if dtype == "bf16" and not swiglu else []
+    for row in large:                                        # products with 16 + code pass 2^128, their sums here do not
+        x[row] = (clean[row].float() * 2.0 ** 122).bfloat16()
+    out = tops.expert_linear_w4(x, tokens, packed, swiglu=swiglu)
+    ref = tops.expert_linear_w4(clean, tokens, packed, swiglu=swiglu)
+    rest = torch.tensor([r not in bad and r not in large for r in range(P)], device=DEV)
+    assert same(out[rest], ref[rest])
+    for row in [*bad, *large]:
+        xd = x[row].double()
+        want = (xd * weight[expert[row]]).sum(-1)
+        if swiglu:
+            g, u = want[:N // 2], want[N // 2:]
+            want = g * torch.sigmoid(g) * u
+        got, inf = out[row].double(), want.isinf()
+        assert torch.equal(got.isnan(), want.isnan()), row
+        assert torch.equal(got[inf], want[inf]), row
+        fin = want.isfinite()
+        if row in large:
+            assert bool(fin.all())
+            near(out[row], want, xd.abs() @ size[expert[row]].T, K + 2 * (group + 2) + K / group + 10, "large")
+        else:                                                # one infinity or NaN reaches every result of its row
+            assert not bool(fin.any())
