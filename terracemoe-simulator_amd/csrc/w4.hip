@@ -665,8 +665,12 @@ __global__ __launch_bounds__(4 * kWave, 2) void w4_many_kernel(W4Args a) {
     }
 }
 
+// HIP launches up to 2^32 - 1 threads.  The tiled kernel takes 256 for 256 columns of 32 or 64 rows, the few-row kernel 64
+// for 32 columns of 16 rows where there are many, so only a great number of experts of a few rows each passes the limit.
+static bool w4_fits(int64_t blocks, int threads) { return blocks * threads < (int64_t)1 << 32; }
+
 template <int DT, bool ZEROS>
-static void launch_w4(W4Args a, int64_t busy, hipStream_t s) {
+static int launch_w4(W4Args a, int64_t busy, hipStream_t s) {
     const int64_t P = a.P;
     // row tiles: the most there can be, and one for rows without an expert
     auto tiles = [&](int64_t R) { return busy + (P - busy) / R + 1; };
@@ -675,6 +679,7 @@ static void launch_w4(W4Args a, int64_t busy, hipStream_t s) {
     const int64_t per_wide = kManyTiles * (a.swiglu ? 32 : 64), wide = (a.out_cols + per_wide - 1) / per_wide;
     if (mean > 8 && wide * (tiles(16 * mt) - 1) >= 256) {
         a.col_blocks = (int)wide;
+        if (!w4_fits(wide * tiles(16 * mt), 4 * kWave)) return TERRACE_EINVAL;
         const unsigned grid = (unsigned)(wide * tiles(16 * mt));
 #define TERRACE_MANY(MT)                                                                            \
     if (a.sh.group == 128) w4_many_kernel<DT, MT, 4, ZEROS><<<grid, 4 * kWave, 0, s>>>(a);          \
@@ -683,7 +688,7 @@ static void launch_w4(W4Args a, int64_t busy, hipStream_t s) {
         if (mt == 2) { TERRACE_MANY(2); }
         else { TERRACE_MANY(4); }
 #undef TERRACE_MANY
-        return;
+        return check_launch();
     }
     const int64_t sets = a.swiglu ? (a.out_cols + 15) / 16 : (a.out_cols + 31) / 32, n = sets * (tiles(16) - 1);
     a.split = 1;
@@ -692,10 +697,12 @@ static void launch_w4(W4Args a, int64_t busy, hipStream_t s) {
     a.per = (a.full + a.split - 1) / a.split;
     a.sets = waves / a.split;
     a.col_blocks = (int)((sets + a.sets - 1) / a.sets);
+    if (!w4_fits(a.col_blocks * tiles(16), waves * kWave)) return TERRACE_EINVAL;
     const unsigned grid = (unsigned)(a.col_blocks * tiles(16)), threads = (unsigned)(waves * kWave);
     if (a.sh.group == 128) w4_few_kernel<DT, 4, ZEROS><<<grid, threads, 0, s>>>(a);
     else if (a.sh.group == 64) w4_few_kernel<DT, 2, ZEROS><<<grid, threads, 0, s>>>(a);
     else w4_few_kernel<DT, 1, ZEROS><<<grid, threads, 0, s>>>(a);
+    return check_launch();
 }
 
 int run_w4_linear(const void *x, int dtype, int64_t P, const int64_t *counts, const void *codes, const void *scales,
@@ -710,18 +717,12 @@ int run_w4_linear(const void *x, int dtype, int64_t P, const int64_t *counts, co
         return TERRACE_EINVAL;
     const int64_t busy = P < n_experts ? P : n_experts;      // experts that can hold a row
     const int64_t out_cols = swiglu ? N / 2 : N;
-    // HIP's grid limit: 2^32 threads, 512 in a workgroup, each at least 16 columns of 16 rows
-    if ((out_cols + 15) / 16 * (busy + (P - busy) / 16 + 1) >= (int64_t)1 << 23) return TERRACE_EINVAL;
     const W4Args a{x, counts, (int)P, sh, (const u32x4 *)codes, (const uint16_t *)scales, (const uint8_t *)zeros, swiglu,
                    out, (int)out_cols, (int)sh.tiles(), (int)sh.blocks(), (int)(K / kBlockK), (int)(K % kBlockK / 32), 1, 1,
                    1, 1};
-#define TERRACE_W4(DT)                              \
-    if (zeros) launch_w4<DT, true>(a, busy, s);     \
-    else launch_w4<DT, false>(a, busy, s)
-    if (dtype == TERRACE_BF16) { TERRACE_W4(TERRACE_BF16); }
-    else { TERRACE_W4(TERRACE_F16); }
-#undef TERRACE_W4
-    return check_launch();
+    if (dtype == TERRACE_BF16)
+        return zeros ? launch_w4<TERRACE_BF16, true>(a, busy, s) : launch_w4<TERRACE_BF16, false>(a, busy, s);
+    return zeros ? launch_w4<TERRACE_F16, true>(a, busy, s) : launch_w4<TERRACE_F16, false>(a, busy, s);
 }
 
 }  // namespace terrace

@@ -154,3 +154,24 @@ def test_w4_products_of_rows_that_are_not_finite_or_very_large(E, N, K, group, z
             near(out[row], want, xd.abs() @ size[expert[row]].T, K + 2 * (group + 2) + K / group + 10, "large")
         else:                                                # one infinity or NaN reaches every result of its row
             assert not bool(fin.any())
+
+
+def test_w4_products_of_a_long_prompt():
+    """300000 rows over 256 experts of 7168 columns: more 16 x 16 tiles than one launch has workgroups, in far fewer of the
+    tiles that run."""
+    import terrace.ops as tops
+    E, N, K, P = 256, 7168, 32, 300_000
+    announce("w4 long", E, N, K, P)
+    codes, scales, _, weight, size = w4_case(E, N, K, 32, "bf16", False, 1)
+    packed = tops.w4_pack(codes, scales)
+    counts = torch.randint(1000, 1300, (E,), generator=gen(2), device=DEV)
+    live = int(counts.sum())
+    assert live < P - 100
+    x = torch.randn((P, K), generator=gen(3), device=DEV).bfloat16()
+    out = tops.expert_linear_w4(x, counts, packed)
+    assert out.shape == (P, N) and not bool(out[live:].any())
+    ends = torch.cumsum(counts, 0)
+    for row in (0, int(ends[0]) - 1, int(ends[0]), 131_071, 131_072, live - 1):
+        e = int(torch.searchsorted(ends, torch.tensor([row], device=DEV), right=True))
+        xd = x[row].double()
+        near(out[row], xd @ weight[e].T, xd.abs() @ size[e].T, 2 * 34 + 1 + 10, f"row {row}")
