@@ -251,13 +251,40 @@ def expert_unsort(rows, weights, plan: ExpertPlan, out_dtype=None):
 
 class W4Weights:
     """4-bit weights laid out for :func:`expert_linear_w4` by :func:`w4_pack`: ``n_experts`` matrices [N, K] in groups of
-    ``group`` along K, for rows of ``dtype``."""
+    ``group`` along K, for rows of ``dtype``.
 
-    __slots__ = ("codes", "scales", "zeros", "n_experts", "N", "K", "group", "dtype", "device")
+    To store them, keep the planes ``codes``, ``scales`` and ``zeros`` (None: 8 everywhere) with the five numbers and the
+    dtype, and hand them to the constructor again; the layout is this build's own.  The planes are checked against the
+    numbers by the first product after any attribute was set; resizing a plane's storage behind it is not seen."""
+
+    __slots__ = ("codes", "scales", "zeros", "n_experts", "N", "K", "group", "dtype", "device", "_sound")
 
     def __init__(self, codes, scales, zeros, n_experts, N, K, group, dtype):
         self.codes, self.scales, self.zeros = codes, scales, zeros
         self.n_experts, self.N, self.K, self.group, self.dtype, self.device = n_experts, N, K, group, dtype, codes.device
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_sound", False)
+
+    def check(self):
+        """Raises RuntimeError unless the planes are what :func:`w4_pack` lays out for these sizes."""
+        if self.dtype not in (torch.bfloat16, torch.float16):
+            raise RuntimeError(f"W4Weights: bfloat16 or float16, got {self.dtype}")
+        planes = (("codes", self.codes, torch.uint8, 1, 16), ("scales", self.scales, self.dtype, 2, 8),
+                  ("zeros", self.zeros, torch.uint8, 1, 8))
+        for what, (name, t, dtype, width, boundary) in enumerate(planes):
+            if t is None and name == "zeros":
+                continue
+            need = _hip.query("terrace_w4_packed_bytes", self.n_experts, self.N, self.K, self.group, what)
+            if not need:
+                raise RuntimeError(f"W4Weights: {self.n_experts} matrices of {self.N} x {self.K} in groups of {self.group} are "
+                                   f"not taken")
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.numel() * width != need or not t.is_contiguous() or \
+                    t.device != self.device or t.data_ptr() % boundary:
+                raise RuntimeError(f"W4Weights: {name} must hold {need} bytes of {dtype}, packed, on {self.device} and a "
+                                   f"{boundary}-byte boundary, as w4_pack lays them out")
+        object.__setattr__(self, "_sound", True)
 
 
 def w4_pack(codes, scales, zeros=None) -> W4Weights:
@@ -310,6 +337,8 @@ def expert_linear_w4(rows, tokens_per_expert, weights: W4Weights, swiglu: bool =
     raises."""
     w = weights
     index = _ready(rows, tokens_per_expert, w.codes)
+    if not w._sound:
+        w.check()
     if rows.dim() != 2 or rows.shape[1] != w.K or rows.dtype != w.dtype:
         raise RuntimeError(f"expert_linear_w4: rows must be {w.dtype} [P, {w.K}], got {rows.dtype} {tuple(rows.shape)}")
     if tokens_per_expert is None:

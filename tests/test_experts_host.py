@@ -163,3 +163,35 @@ def test_a_forward_mode_tangent_is_refused_by_the_operators_of_the_path_that_car
         for f in calls:
             with pytest.raises(RuntimeError, match="forward-mode"):
                 f()
+
+
+def test_planes_that_do_not_fit_the_sizes_are_refused():
+    """A product reads what the sizes say, so a handle built by hand is checked before its first one."""
+    import terrace.ops as tops
+    E, N, K, g = 2, 40, 160, 32                              # 3 column tiles, 2 blocks of k
+
+    def planes(dtype=torch.bfloat16):
+        return (torch.zeros(E * 48 * 2 * 64, dtype=torch.uint8), torch.zeros(E * 48 * 8, dtype=dtype),
+                torch.zeros(E * 48 * 8, dtype=torch.uint8))
+
+    c, s, z = planes()
+    good = tops.W4Weights(c, s, z, E, N, K, g, torch.bfloat16)
+    good.check()
+    tops.W4Weights(c, s, None, E, N, K, g, torch.bfloat16).check()
+    tops.W4Weights(c.view(E, 3, 2, 64, 16), s.view(E, -1), z, E, N, K, g, torch.bfloat16).check()
+    odd = torch.zeros(c.numel() + 1, dtype=torch.uint8)[1:]
+    for bad in ((c[:-1], s, z, E, N, K, g, torch.bfloat16), (c, s[:-8], z, E, N, K, g, torch.bfloat16),
+                (c, s, z[:-8], E, N, K, g, torch.bfloat16), (c, s, z, E + 1, N, K, g, torch.bfloat16),
+                (c, s, z, E, N + 16, K, g, torch.bfloat16), (c, s, z, E, N, K + 128, g, torch.bfloat16),
+                (c, s, z, E, N, K, 64, torch.bfloat16), (c, s, z, E, N, 1 << 40, g, torch.bfloat16),
+                (c, s, z, E, N, K, g, torch.float16), (c, s.float(), z, E, N, K, g, torch.float32),
+                (c, None, z, E, N, K, g, torch.bfloat16), (c.view(torch.int8), s, z, E, N, K, g, torch.bfloat16),
+                (c.repeat_interleave(2)[::2], s, z, E, N, K, g, torch.bfloat16), (odd, s, z, E, N, K, g, torch.bfloat16),
+                (c, s.to("meta"), z, E, N, K, g, torch.bfloat16), (c, s, z, -1, N, K, g, torch.bfloat16)):
+        with pytest.raises(RuntimeError, match="W4Weights"):
+            tops.W4Weights(*bad).check()
+    assert good._sound
+    good.N = 56                                              # a handle that was sound is looked at again after a change
+    assert not good._sound
+    with pytest.raises(RuntimeError, match="W4Weights"):
+        good.check()

@@ -175,3 +175,21 @@ def test_w4_products_of_a_long_prompt():
         e = int(torch.searchsorted(ends, torch.tensor([row], device=DEV), right=True))
         xd = x[row].double()
         near(out[row], xd @ weight[e].T, xd.abs() @ size[e].T, 2 * 34 + 1 + 10, f"row {row}")
+
+
+def test_a_handle_of_4_bit_weights_stored_and_built_again():
+    import terrace.ops as tops
+    announce("w4 handle")
+    codes, scales, z, _, _ = w4_case(3, 40, 160, 32, "f16", True, 9)
+    w = tops.w4_pack(codes, scales, z)
+    x, counts = torch.randn((7, 160), generator=gen(1), device=DEV).half(), torch.tensor([3, 0, 4], device=DEV)
+    want = tops.expert_linear_w4(x, counts, w)
+    planes = [t.cpu().to(DEV) for t in (w.codes, w.scales, w.zeros)]
+    again = tops.W4Weights(*planes, w.n_experts, w.N, w.K, w.group, w.dtype)
+    assert torch.equal(tops.expert_linear_w4(x, counts, again), want)
+    for name, value in (("N", 56), ("n_experts", 4), ("codes", planes[0][:-1024]), ("zeros", planes[2][1:])):
+        bad = tops.W4Weights(*planes, w.n_experts, w.N, w.K, w.group, w.dtype)
+        tops.expert_linear_w4(x, counts, bad)
+        setattr(bad, name, value)
+        with pytest.raises(RuntimeError, match="W4Weights"):
+            tops.expert_linear_w4(x, counts if name != "n_experts" else torch.tensor([3, 0, 4, 0], device=DEV), bad)
