@@ -27,9 +27,15 @@ int run_expert_index(const int64_t *expert_idx, int64_t P, int n_experts, int64_
 // launch: what bounds it is the latency of one launch and two dependent reads (the ids, then nothing but stores).
 // 8 experts of 256 a token, 14 KB rows, against the sorting path: 32 tokens 4.7 us for 9.8, 128 tokens 7.9 for 10.9, 512
 // tokens 26 for 35, 1024 tokens 62 for 48; one expert a token, 2000 tokens 10.3 for 19.2, 8000 tokens 66 for 17.
+//
+// Every workgroup of a token repeats its ranking, and a row in pieces of a few bytes (an odd width, a base off 16 bytes) has
+// many slices: 28 at 7167 bf16.  So a token gets no more workgroups than 2048 in all need, but four, and each walks on over
+// the row: 512 such tokens 43 us, 111 with a workgroup a slice, where 513 take the sorting path in 53; 2000 tokens of one
+// expert 49 us for 170 (2049: 72); 16 tokens 5.9 us either way.
 static bool few_pairs(int64_t T, int64_t P) { return P <= 2048 || (P <= 4096 && T <= 1024); }
 constexpr int kMaxSmallExperts = kMaxBuckets;
 constexpr int kSmallFan = 16;
+constexpr int kSmallGroups = 2048;
 
 template <typename V>
 __global__ __launch_bounds__(kBlock) void expert_sort_small_kernel(
@@ -68,7 +74,7 @@ __global__ __launch_bounds__(kBlock) void expert_sort_small_kernel(
         return;
     }
     const int t = (int)blockIdx.x / slices, slice = (int)blockIdx.x - t * slices;
-    const int64_t i = (int64_t)slice * kBlock + threadIdx.x;
+    const int64_t i = (int64_t)slice * kBlock + threadIdx.x, step = (int64_t)slices * kBlock;
     V v = zero_of<V>();
     if (rows && i < live_vecs) v = x[(int64_t)t * row_vecs + i];
     for (int j0 = 0; j0 < k; j0 += kSmallFan) {              // one round for k <= 16
@@ -98,11 +104,16 @@ __global__ __launch_bounds__(kBlock) void expert_sort_small_kernel(
             if (lane == j) below[w][j] = n[j];
         }
         __syncthreads();
-        for (int j = 0; j < m; ++j) {
-            const int place = below[0][j] + below[1][j] + below[2][j] + below[3][j];
-            const bool live = read_lane(key, j) < n_experts;
-            if (slice == 0 && threadIdx.x == 0) where[t * k + j0 + j] = live ? place : -1;
-            if (rows && i < live_vecs) rows[(int64_t)place * row_vecs + i] = live ? v : zero_of<V>();
+        const uint64_t alive = __ballot(key < n_experts);
+        if (slice == 0 && w == 0 && lane < m)
+            where[t * k + j0 + lane] = alive >> lane & 1 ? below[0][lane] + below[1][lane] + below[2][lane] + below[3][lane] : -1;
+        V u = v;
+        for (int64_t c = i; rows && c < live_vecs; c += step) {          // once where the slices are the whole row
+            if (c != i) u = x[(int64_t)t * row_vecs + c];
+            for (int j = 0; j < m; ++j) {
+                const int place = below[0][j] + below[1][j] + below[2][j] + below[3][j];
+                rows[(int64_t)place * row_vecs + c] = alive >> j & 1 ? u : zero_of<V>();
+            }
         }
         __syncthreads();
     }
@@ -161,9 +172,8 @@ int run_expert_sort(const void *x, const int64_t *expert_idx, int64_t T, int64_t
     const bool move = x && g.width > 0;
     const int vb = move ? row_vec_bytes(g, x, rows) : 16;
     if (few_pairs(T, P)) {
-        const int64_t vecs = move ? g.width / vb : 1;
-        const int64_t slices = (vecs + kBlock - 1) / kBlock;
-        if (T * slices >= ((int64_t)1 << 31) / kBlock) return TERRACE_EINVAL;
+        const int64_t vecs = move ? g.width / vb : 1, most = kSmallGroups / T > 4 ? kSmallGroups / T : 4;
+        const int64_t need = (vecs + kBlock - 1) / kBlock, slices = need < most ? need : most;
         const unsigned grid = (unsigned)(T * slices + 1);
 #define TERRACE_SMALL(V)                                                                                            \
     expert_sort_small_kernel<V><<<grid, kBlock, 0, s>>>((const V *)x, expert_idx, (int)T, k, n_experts, g.pitch / vb, \

@@ -5,7 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_experts import DEV, DT, announce, gen, near, norm_inputs, routing, w4_case
+from test_gpu_experts import (DEV, DT, announce, check_sort, gen, near, norm_inputs, off_boundary, routing, sort_oracle,
+                              w4_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -193,3 +194,33 @@ def test_a_handle_of_4_bit_weights_stored_and_built_again():
         setattr(bad, name, value)
         with pytest.raises(RuntimeError, match="W4Weights"):
             tops.expert_linear_w4(x, counts if name != "n_experts" else torch.tensor([3, 0, 4, 0], device=DEV), bad)
+
+
+# ---- the one-launch sort of rows of many pieces ---------------------------------------------------------------------
+@pytest.mark.parametrize("T,k,H,dtype,off", [
+    (512, 8, 7167, "bf16", False), (512, 8, 7168, "bf16", True), (1, 8, 40001, "f16", False), (1000, 4, 2049, "f32", False),
+    (1000, 4, 5000, "f32", True), (2048, 1, 9001, "bf16", False), (120, 17, 4099, "f16", False), (3, 40, 3001, "f32", True),
+    (513, 8, 1001, "bf16", False), (1025, 4, 515, "f16", True), (3000, 3, 1001, "f32", True), (2100, 2, 7167, "bf16", False),
+])
+def test_expert_sort_rows_of_many_pieces(T, k, H, dtype, off):
+    """Odd widths and bases off a boundary, where a row is moved in pieces of few bytes; both the one-launch form, whose
+    workgroups then take several pieces each, and the sorting path."""
+    announce("expert_sort pieces", T, k, H, dtype, off)
+    x = torch.randn((T, H), generator=gen(T + H), device=DEV).to(DT[dtype])
+    check_sort(off_boundary(x) if off else x, routing(T, 60, k, T, 0.1), 60)
+
+
+def test_expert_sort_rows_of_megabytes():
+    """2048 rows of a million and one elements of two bytes: 4097 pieces a row."""
+    import terrace.ops as tops
+    T, H = 2048, 1_048_577
+    announce("expert_sort megabytes", T, H)
+    x = torch.randint(-30000, 30000, (T, H), generator=gen(1), device=DEV, dtype=torch.int16)
+    idx = routing(T, 16, 1, 2, 0.1)
+    rows, plan = tops.expert_sort(x, idx, 16)
+    where, _, offsets = sort_oracle(idx, 16)
+    assert torch.equal(plan.where.cpu(), where)
+    live = (where[:, 0] >= 0).nonzero()[:, 0].to(DEV)
+    for part in live.split(256):
+        assert torch.equal(rows[plan.where[part, 0]], x[part])
+    assert not bool(rows[int(offsets[-1]):].any())
