@@ -513,7 +513,7 @@ TERRACE_API int terrace_expert_sort(const void *x, const int64_t *expert_idx, in
  * in fp32, each rounded once.  rows and d_rows [n_rows,hidden] of row_dtype, dy [T,hidden] of dy_dtype, weights and
  * d_weights [T,k] of w_dtype (F32, BF16, F16); weights NULL: all ones.  d_rows or d_weights may be NULL (not wanted;
  * rows is read for d_weights only).  Rows of d_rows from *n_live on (offsets[n_experts] of the plan, device memory)
- * are written as zeros. */
+ * are written as zeros.  T is at most 2^24 - 1025 (one workgroup a token). */
 TERRACE_API int terrace_expert_unsort_grad(const void *rows, int row_dtype, const void *dy, int dy_dtype,
                                            const int64_t *where, const void *weights, int w_dtype, int64_t T, int k,
                                            int64_t hidden, int64_t n_rows, const int64_t *n_live, void *d_rows,

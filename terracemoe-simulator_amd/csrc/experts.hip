@@ -374,8 +374,8 @@ int run_expert_unsort_grad(const void *src, int src_dtype, const void *dy, int d
                            const int64_t *live, void *d_rows, void *d_weights, hipStream_t s) {
     auto is_float = [](int d) { return d == TERRACE_F32 || d == TERRACE_BF16 || d == TERRACE_F16; };
     if (T < 0 || k <= 0 || hidden < 0 || n_rows < 0 || !is_float(src_dtype) || !is_float(dy_dtype) ||
-        !is_float(w_dtype) || T > (((int64_t)1 << 31) - 1) / k || T + kTailBlocks >= ((int64_t)1 << 31) / kBlock)
-        return TERRACE_EINVAL;
+        !is_float(w_dtype) || T > (((int64_t)1 << 31) - 1) / k || T + kTailBlocks >= ((int64_t)1 << 32) / kBlock)
+        return TERRACE_EINVAL;                               // a launch has fewer than 2^32 threads
     if (!d_rows && !d_weights) return TERRACE_OK;
     if (T == 0 && n_rows == 0) return TERRACE_OK;
     if ((T && (!where || (hidden && (!dy || (d_weights && n_rows && !src))))) || (d_rows && !live)) return TERRACE_EINVAL;

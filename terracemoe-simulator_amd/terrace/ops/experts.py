@@ -19,6 +19,7 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _CODE = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16, torch.float16: _hip.F16}
 _MAX_EXPERTS = 2048
 _MAX_WIDTH = 16384
+_MAX_GRAD_TOKENS = (1 << 24) - 1025          # one workgroup a token and 1024 for the rows of none, below 2^32 threads
 _CURRENT = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -228,7 +229,7 @@ def expert_unsort(rows, weights, plan: ExpertPlan, out_dtype=None):
     ``rows`` [T*k, H] float32 / bfloat16 / float16 in the order of ``plan`` (a plan of :func:`expert_sort`),
     ``weights`` [T, k] of any of these types, or None for plain sums.  A pair without an expert contributes nothing and
     a token without any is a zero row, whatever ``rows`` holds behind the live rows.  Carries gradients to ``rows``
-    (zeros behind the live rows) and ``weights`` (0 where there is no expert)."""
+    (zeros behind the live rows) and ``weights`` (0 where there is no expert), for up to 2^24 - 1025 tokens."""
     index = _ready(rows, weights, plan.planes)
     T, k = plan.T, plan.k
     out_dtype = out_dtype or rows.dtype
@@ -241,6 +242,8 @@ def expert_unsort(rows, weights, plan: ExpertPlan, out_dtype=None):
     rows = rows.contiguous()
     weights = None if weights is None else weights.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+        if T > _MAX_GRAD_TOKENS:
+            raise RuntimeError(f"expert_unsort: gradients for up to {_MAX_GRAD_TOKENS} tokens, got {T}")
         return _ExpertUnsortFn.apply(rows, weights, plan.planes, T, k, plan.n_experts, out_dtype)
     return _combine(index, rows, plan.planes.data_ptr(), weights, T, k, out_dtype)
 

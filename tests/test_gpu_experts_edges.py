@@ -224,3 +224,36 @@ def test_expert_sort_rows_of_megabytes():
     for part in live.split(256):
         assert torch.equal(rows[plan.where[part, 0]], x[part])
     assert not bool(rows[int(offsets[-1]):].any())
+
+
+# ---- many tokens --------------------------------------------------------------------------------------------------
+def test_expert_unsort_gradient_of_nine_million_tokens():
+    """As many as the forward call takes: more workgroups than 2^31 threads."""
+    import terrace.ops as tops
+    T, H = 9_000_000, 8
+    announce("expert_unsort tokens", T, H)
+    idx = torch.randint(-1, 5, (T, 1), generator=gen(1), device=DEV)
+    _, plan = tops.expert_sort(torch.zeros((T, 0), device=DEV), idx, 5)
+    rows = torch.randn((T, H), generator=gen(2), device=DEV).bfloat16().requires_grad_(True)
+    weights = torch.rand((T, 1), generator=gen(3), device=DEV).bfloat16().requires_grad_(True)
+    dy = torch.randn((T, H), generator=gen(4), device=DEV).bfloat16()
+    y = tops.expert_unsort(rows, weights, plan)
+    d_rows, d_w = torch.autograd.grad(y, (rows, weights), dy)
+    live, at = plan.where[:, 0] >= 0, plan.where[:, 0].clamp(min=0)
+    want = torch.where(live[:, None], rows.detach().double()[at] * weights.detach().double(), 0.0)
+    near(y.detach(), want, want.abs(), 2, "y")
+    want = torch.zeros((T, H), device=DEV)
+    want[at[live]] = (weights.detach().float() * dy.float())[live]
+    near(d_rows, want.double(), want.double().abs(), 1, "d_rows")
+    terms = torch.where(live[:, None], rows.detach().double()[at] * dy.double(), 0.0)
+    near(d_w, terms.sum(1, keepdim=True), terms.abs().sum(1, keepdim=True), H + 10, "d_weights")
+
+
+def test_expert_unsort_refuses_a_gradient_it_could_not_compute():
+    import terrace.ops as tops
+    T = (1 << 24) - 1024
+    announce("expert_unsort tokens refused", T)
+    plan = tops.ExpertPlan(torch.full((T + 2 * 2 + 3,), -1, dtype=torch.int64, device=DEV), T, 1, 2)
+    rows = torch.zeros((T, 1), dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="gradients for up to"):
+        tops.expert_unsort(rows, None, plan)
