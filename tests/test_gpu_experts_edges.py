@@ -5,8 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_experts import (DEV, DT, announce, check_sort, gen, near, norm_inputs, off_boundary, routing, sort_oracle,
-                              w4_case)
+from test_gpu_experts import (DEV, DT, announce, check_norm, check_sort, gen, near, norm_inputs, off_boundary, routing,
+                              sort_oracle, w4_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -80,6 +80,27 @@ def test_block_norm_gradient_of_h_alone_on_very_large_values(dtype, gate):
         near(dg, terms.sum(1, keepdim=True), terms.abs().sum(1, keepdim=True), H / 64 + 40, "d_gate")
     else:
         near(dg, terms.sum(0), terms.abs().sum(0), T + 40, "d_gate")
+
+
+# ---- block_norm over more rows than are fetched one ahead ----------------------------------------------------------
+@pytest.mark.parametrize("H", [7168, 7167, 8200, 8195])
+@pytest.mark.parametrize("dtype,residual", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("T,gate", [(2049, "token"), (2900, "channel")])
+def test_block_norm_of_long_walks(T, H, dtype, residual, gate):
+    """More than 2048 groups of rows: every type with aligned and unaligned rows, 8 and 16 elements a lane, a gate per
+    token riding with the rows, and walks that end after an odd and after an even number of rows."""
+    check_norm(T, H, dtype, residual, True, True, gate, True, seed=T + H)
+
+
+@pytest.mark.parametrize("T,H,dtype,residual,has_y,post,gate,pre", [
+    (33000, 264, "f16", "f32", True, True, "token", True), (36900, 33, "bf16", "bf16", True, True, "token", False),
+    (4200, 4096, "f32", "f32", True, False, "channel", True), (4100, 4095, "f16", "f16", True, True, "token", False),
+    (16500, 1000, "bf16", "f32", True, False, "token", True), (2051, 7168, "bf16", "bf16", True, True, None, False),
+    (2600, 8000, "f32", "f32", False, False, None, True), (2300, 16384, "f32", "f32", True, False, None, True),
+    (2100, 16383, "bf16", "bf16", False, False, None, True), (2561, 9000, "f16", "f32", True, True, "token", False),
+])
+def test_block_norm_of_long_walks_with_one_norm_and_several_rows_a_workgroup(T, H, dtype, residual, has_y, post, gate, pre):
+    check_norm(T, H, dtype, residual, has_y, post, gate, pre, seed=T + H)
 
 
 # ---- forward mode -------------------------------------------------------------------------------------------------
