@@ -174,9 +174,16 @@ __device__ __forceinline__ void row_sum(float *v, float *part, int tpr) {
 
 // A workgroup walks the rows (blockIdx.x + i * gridDim.x) * groups + group, with rows in flight while its waves meet: the next
 // one, fetched at the start of a row (AHEAD 1), or the next two, a row's registers taking the row after the next as soon
-// as h is made of them (AHEAD 2).  16384 rows of 7168 bf16, 940 MB, 64 rows a workgroup: 162 us with two (5.8 TB/s), 173-183
-// us with one, 287 us with none and a workgroup a row.  Over few rows the two do not differ beyond the noise (4096 f32 rows of
-// 1024: 16-20 us) and one takes fewer registers.
+// as h is made of them (AHEAD 2).  16384 rows of 7168 bf16, 940 MB, 64 rows a workgroup: 162-170 us with two (5.8 TB/s),
+// 173-183 us with one, 287 us with none and a workgroup a row.  Two ahead are taken over more than 2048 groups of rows where a
+// row's bits are few, that is 16-bit rows beside a 16-bit residual, and not both unaligned and 16 elements a lane
+// (norm_two_ahead); two / one ahead, us:
+//   taken      16384 x 12288 bf16 290 / 304, x 16384 406 / 415, x 7167 361 / 383; 4096 x 7168 47.4 / 47.9, x 16384 101 / 100
+//   not taken  16384 x 7168 beside f32 283 / 268, f32 388 / 362; x 16384 beside f32 667 / 633, f32 986 / 849; x 12289 bf16 499 / 448
+// (the f32 and the unaligned wide forms with two ahead spill 14 to 83 registers a lane).  Over fewer groups one is as fast
+// or faster: 4096 x 1024 bf16 10.9 / 9.9, f32 19 / 17.
+constexpr bool norm_two_ahead(int r_dtype, bool aligned, int per) { return r_dtype != TERRACE_F32 && (aligned || per == 8); }
+
 template <int TY, int TR, bool ALIGNED, int E, int AHEAD>
 __global__ __launch_bounds__(kNormThreads) void block_norm_kernel(NormArgs a, void *__restrict__ h_out,
                                                                   void *__restrict__ n_out, float *__restrict__ stats) {
@@ -562,8 +569,9 @@ int run_block_norm(const void *y, int y_dtype, const void *residual, int r_dtype
     const int64_t need = (T + a.groups - 1) / a.groups;
     const unsigned grid = (unsigned)(need < kNormBlocks ? need : kNormBlocks), threads = (unsigned)(a.tpr * a.groups);
 #define TERRACE_NORM_AHEAD(Y, R, A, E)                                                                     \
-    if (need <= 8 * kNormBlocks) block_norm_kernel<Y, R, A, E, 1><<<grid, threads, 0, s>>>(a, h, n, stats);    \
-    else block_norm_kernel<Y, R, A, E, 2><<<grid, threads, 0, s>>>(a, h, n, stats)
+    if (norm_two_ahead(R, A, E) && need > 8 * kNormBlocks)                                                 \
+        block_norm_kernel<Y, R, A, E, norm_two_ahead(R, A, E) ? 2 : 1><<<grid, threads, 0, s>>>(a, h, n, stats); \
+    else block_norm_kernel<Y, R, A, E, 1><<<grid, threads, 0, s>>>(a, h, n, stats)
 #define TERRACE_NORM(Y, R)                                                     \
     if (form.aligned && form.per == 8) { TERRACE_NORM_AHEAD(Y, R, true, 8); }  \
     else if (form.aligned) { TERRACE_NORM_AHEAD(Y, R, true, 16); }             \
