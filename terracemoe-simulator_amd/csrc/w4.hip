@@ -543,8 +543,19 @@ __global__ __launch_bounds__(kMaxSplit * kWave) void w4_few_kernel(W4Args a) {
 // instructions take them, while every wave streams its own codes two blocks ahead.  2048 rows over 64 experts of 4096 x
 // 4096 199-211 us (0.33 PFLOP/s, 612 MB), 256 rows of each of 8 experts 85-90 us.  By counters vector instructions (307 a block
 // and wave, and the issue of 40 matrix instructions) fill 60 % of the cycles and matrix instructions 28 %: neither is full, and two
-// waves a SIMD do not hide one behind the other.  From more than 8 rows a busy expert on it beats the kernel above: 1024
-// rows over 64 experts of 2048 x 7168 141 us for 194.
+// waves a SIMD do not hide one behind the other.
+//
+// Against the kernel above (few / tiled, us, without and with zero points): 64 experts of 2048 x 7168, 4 rows each 94 / 99
+// and 100 / 114, 8 rows 105 / 100 and 112 / 114, 16 rows 135 / 102 and 141 / 117; of 4096 x 4096 8 rows 116 / 129 and 123 / 138,
+// 12 rows 133 / 132 and 143 / 138, 16 rows 150 / 134 and 157 / 139; 256 experts of 7168 x 2048, 8 rows 447 / 399 and
+// 465 / 475.  So it is taken from more than 8 rows a busy expert on, and where its grid holds a workgroup for every CU:
+// with half of them, 8 experts of 4096 x 4096, 16 rows 27 / 34 and 27 / 41 and 32 rows 42 / 35 and 45 / 42; with an eighth to a
+// quarter, one matrix of 7168 x 7168 at 64 rows 37 / 87, of 16384 x 4096 43 / 54.
+//
+// MT 4 reads and expands the codes once for 64 rows, at up to 250 registers; with zero points it does not fit them.  32 / 64
+// rows a tile: 8 experts of 4096 x 4096, groups of 64, 64 rows each 37 / 73 us, 128 rows 54 / 58, 256 rows 96 / 87; 32 experts of
+// 2048 x 7168, 64 rows 91 / 94, 128 rows 173 / 153, 256 rows 327 / 299.  With zero points 64 rows 99 / 194, 128 rows 193 / 245,
+// 256 rows 384 / 495 (spilling): not built.
 constexpr int kManyTiles = 4;
 // (two waves a SIMD at least: with a whole SIMD's registers to itself the compiler puts the sums into accumulation
 // registers and copies each out again before the multiply-add, a fifth of the kernel's instructions)
@@ -675,7 +686,7 @@ static int launch_w4(W4Args a, int64_t busy, hipStream_t s) {
     // row tiles: the most there can be, and one for rows without an expert
     auto tiles = [&](int64_t R) { return busy + (P - busy) / R + 1; };
     const int64_t mean = (P + busy - 1) / busy;
-    const int mt = mean <= 32 ? 2 : 4;
+    const int mt = !ZEROS && mean >= 128 ? 4 : 2;
     const int64_t per_wide = kManyTiles * (a.swiglu ? 32 : 64), wide = (a.out_cols + per_wide - 1) / per_wide;
     if (mean > 8 && wide * (tiles(16 * mt) - 1) >= 256) {
         a.col_blocks = (int)wide;
@@ -685,8 +696,13 @@ static int launch_w4(W4Args a, int64_t busy, hipStream_t s) {
     if (a.sh.group == 128) w4_many_kernel<DT, MT, 4, ZEROS><<<grid, 4 * kWave, 0, s>>>(a);          \
     else if (a.sh.group == 64) w4_many_kernel<DT, MT, 2, ZEROS><<<grid, 4 * kWave, 0, s>>>(a);      \
     else w4_many_kernel<DT, MT, 1, ZEROS><<<grid, 4 * kWave, 0, s>>>(a)
-        if (mt == 2) { TERRACE_MANY(2); }
-        else { TERRACE_MANY(4); }
+        if constexpr (!ZEROS) {
+            if (mt == 4) {
+                TERRACE_MANY(4);
+                return check_launch();
+            }
+        }
+        TERRACE_MANY(2);
 #undef TERRACE_MANY
         return check_launch();
     }

@@ -5,8 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_experts import (DEV, DT, announce, check_norm, check_sort, gen, near, norm_inputs, off_boundary, routing,
-                              sort_oracle, w4_case)
+from test_gpu_experts import (DEV, DT, announce, check_norm, check_sort, check_w4, gen, near, norm_inputs, off_boundary,
+                              routing, sort_oracle, w4_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -176,6 +176,17 @@ def test_w4_products_of_rows_that_are_not_finite_or_very_large(E, N, K, group, z
             near(out[row], want, xd.abs() @ size[expert[row]].T, K + 2 * (group + 2) + K / group + 10, "large")
         else:                                                # one infinity or NaN reaches every result of its row
             assert not bool(fin.any())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("E,N,K,group,zeros,swiglu,counts", [
+    (1, 16400, 192, 64, False, False, [200]), (2, 16400, 256, 128, False, True, [140, 130]), (1, 16390, 160, 32, False, False, [129]),
+    (2, 24010, 320, 64, False, False, [128, 128]), (2, 24010, 320, 64, False, True, [127, 127]),      # 64 rows a tile, and 32
+    (1, 16400, 192, 64, True, False, [200]), (2, 16400, 256, 128, True, True, [140, 130]),            # zero points: 32
+    (3, 22000, 96, 32, True, False, [9, 9, 9]), (33, 2048, 64, 64, False, False, [8] * 33), (33, 2048, 64, 64, False, True, [9] * 33),
+])
+def test_w4_products_on_both_sides_of_each_choice_of_kernel(E, N, K, group, zeros, swiglu, counts, dtype):
+    check_w4(E, N, K, group, dtype, zeros, swiglu, counts, 5, E + N)
 
 
 def test_w4_products_of_a_long_prompt():
