@@ -632,47 +632,65 @@ __global__ __launch_bounds__(4 * kWave, 2) void w4_many_kernel(W4Args a) {
         }
     }
     if (b < blocks) use(0);
-    // the results of a lane in pairs: tiles 2p and 2p + 1, with `swiglu` a gate and its partner; the lane's place is worked
-    // out again here, so that nothing of it is kept over the loop
+    // the sums and the lane's place are taken up anew here: kept in view over the loop, what follows it costs the loop
+    // registers (one form spilled ten)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < T; ++t) asm volatile("" : "+v"(total[m][t]));
     int late = lane;
     asm volatile("" : "+v"(late));
     const int row0 = 4 * (late >> 4), col0 = late & 15;
-    uint32_t again = 0;                                      // pairs with a sum that is not finite
-    auto store = [&](int row, int c0, int c1, float v0, float v1) {
-        uint16_t *o = (uint16_t *)a.out + (int64_t)(rt.first + row) * a.out_cols;
-        if (a.swiglu) {
-            if (c0 < a.out_cols) o[c0] = (uint16_t)to_bits16<DT>(w4_swiglu(v0, v1));
-        } else {
-            if (c0 < a.out_cols) o[c0] = (uint16_t)to_bits16<DT>(v0);
-            if (c1 < a.out_cols) o[c1] = (uint16_t)to_bits16<DT>(v1);
-        }
-    };
+    float poison[4] = {0.0f, 0.0f, 0.0f, 0.0f};              // NaN from the first sum that is not finite on
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) poison[i] = __fmaf_rn(total[m][t][i], 0.0f, poison[i]);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = 16 * m + i + row0;
             if (row >= rt.rows) continue;
+            uint16_t *o = (uint16_t *)a.out + (int64_t)(rt.first + row) * a.out_cols;
+            if (a.swiglu) {
 #pragma unroll
-            for (int p = 0; p < T / 2; ++p) {
-                const float v0 = total[m][2 * p][i], v1 = total[m][2 * p + 1][i];
-                if (!w4_finite(v0) || !w4_finite(v1)) again |= 1u << ((m * 4 + i) * (T / 2) + p);
-                store(row, column(2 * p) + col0, column(2 * p + 1) + col0, v0, v1);
+                for (int t = 0; t < T; t += 2)
+                    if (column(t) + col0 < a.out_cols)
+                        o[column(t) + col0] = (uint16_t)to_bits16<DT>(w4_swiglu(total[m][t][i], total[m][t + 1][i]));
+            } else {
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+                    if (column(t) + col0 < a.out_cols) o[column(t) + col0] = (uint16_t)to_bits16<DT>(total[m][t][i]);
             }
         }
     }
+    if (poison[0] + poison[1] + poison[2] + poison[3] == 0.0f) return;
+    uint32_t again = 0;                                      // pairs of tiles, 2p and 2p + 1, with such a sum: m, i, p in the bits
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int p = 0; p < T / 2; ++p)
+                if (16 * m + i + row0 < rt.rows && !(w4_finite(total[m][2 * p][i]) && w4_finite(total[m][2 * p + 1][i])))
+                    again |= 1u << ((m * 4 + i) * (T / 2) + p);
     for (uint32_t left = again; left; left &= left - 1) {
         const int bit = __builtin_ctz(left), row = bit / (T / 2) / 4 * 16 + bit / (T / 2) % 4 + row0, p = bit % (T / 2);
         const int c0 = column(2 * p) + col0, c1 = column(2 * p + 1) + col0;
         const uint8_t *x = xt + (int64_t)row * a.sh.K * 2;
-        float v[2];
+        uint16_t *o = (uint16_t *)a.out + (int64_t)(rt.first + row) * a.out_cols;
+        float v0 = 0.0f;
 #pragma unroll 1
         for (int j = 0; j < 2; ++j) {
-            const float r = w4_plain<DT, GS, ZEROS>(a, we, j ? c1 : c0, x);
-            v[0] = j ? v[0] : r;
-            v[1] = r;
+            const float v = w4_plain<DT, GS, ZEROS>(a, we, j ? c1 : c0, x);
+            const int c = j ? c1 : c0;
+            if (!a.swiglu && c < a.out_cols) o[c] = (uint16_t)to_bits16<DT>(v);
+            if (a.swiglu && j && c0 < a.out_cols) o[c0] = (uint16_t)to_bits16<DT>(w4_swiglu(v0, v));
+            v0 = v;
         }
-        store(row, c0, c1, v[0], v[1]);
     }
 }
 
