@@ -289,3 +289,65 @@ def test_expert_unsort_refuses_a_gradient_it_could_not_compute():
     rows = torch.zeros((T, 1), dtype=torch.bfloat16, device=DEV, requires_grad=True)
     with pytest.raises(RuntimeError, match="gradients for up to"):
         tops.expert_unsort(rows, None, plan)
+
+
+# ---- layouts ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [60, 3000])
+def test_rows_on_a_kilobyte_pitch_carry_gradients(T):
+    import terrace.ops as tops
+    announce("pitched gradient", T)
+    H, k, E = 480, 3, 7
+    x = torch.randn((T, 512), generator=gen(1), device=DEV).bfloat16()[:, :H].requires_grad_(True)
+    idx = routing(T, E, k, 2, 0.2)
+    rows, plan = tops.expert_sort(x, idx, E)
+    assert rows.stride(0) == 512
+    packed, _ = tops.expert_sort(x.detach().contiguous(), idx, E)
+    assert torch.equal(rows, packed)
+    w = torch.rand((T, k), generator=gen(3), device=DEV).bfloat16()
+    dy = torch.randn((T, H), generator=gen(4), device=DEV).bfloat16()
+    (dx,) = torch.autograd.grad(tops.expert_unsort(rows * 2, w, plan), x, dy)
+    leaf = packed.clone().requires_grad_(True)
+    (d_rows,) = torch.autograd.grad(tops.expert_unsort(leaf * 2, w, plan), leaf, dy)
+    live = plan.where >= 0
+    terms = torch.where(live[..., None], d_rows.double()[plan.where.clamp(min=0)], 0.0)
+    near(dx, terms.sum(1), terms.abs().sum(1), k, "dx")
+
+
+def test_gradients_of_rows_without_width():
+    import terrace.ops as tops
+    announce("no width gradient")
+    idx = routing(30, 8, 2, 1, 0.3)
+    x = torch.zeros((30, 0), device=DEV, requires_grad=True)
+    w = torch.rand((30, 2), generator=gen(2), device=DEV).requires_grad_(True)
+    rows, plan = tops.expert_sort(x, idx, 8)
+    y = tops.expert_unsort(rows, w, plan)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.zeros((30, 0), device=DEV))
+    assert y.shape == dx.shape == (30, 0) and dw.shape == (30, 2) and not bool(dw.any())
+
+
+def test_a_copied_handle_of_4_bit_weights():
+    import copy
+    import pickle
+    import terrace.ops as tops
+    announce("w4 handle copied")
+    codes, scales, _, _, _ = w4_case(1, 32, 64, 32, "bf16", False, 1)
+    w = tops.w4_pack(codes, scales)
+    x = torch.randn((3, 64), generator=gen(1), device=DEV).bfloat16()
+    want = tops.expert_linear_w4(x, None, w)
+    for other in (copy.copy(w), copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert torch.equal(tops.expert_linear_w4(x, None, other), want)
+
+
+def test_function_transforms_are_refused_and_not_ignored():
+    """torch.func hands the operators wrapped tensors, whose memory they cannot address."""
+    import terrace.ops as tops
+    announce("function transforms")
+    x, v = torch.randn((6, 32), generator=gen(1), device=DEV), torch.ones(32, device=DEV)
+    idx = routing(6, 4, 2, 1)
+    for f in (lambda t: tops.block_norm(t, x, v)[0], lambda t: tops.expert_sort(t, idx, 4)[0]):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (x,))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(x)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x[None].expand(2, -1, -1).contiguous())
