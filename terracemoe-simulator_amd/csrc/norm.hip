@@ -261,19 +261,23 @@ __global__ __launch_bounds__(kNormThreads) void block_norm_kernel(NormArgs a, vo
     }
 }
 
-// The gradient: 16384 rows of 7168 bf16, 1.41 GB, in 279 us, 5.0 TB/s.  By counters vector instructions fill
+// The gradient: 16384 rows of 7168 bf16, 1.41 GB, in 271-280 us, 5.0-5.2 TB/s.  By counters vector instructions fill
 // 54 % of the cycles; the 14 waves of a row, alone on their CU, wait for each other once a row, which is likely the rest but
-// was not measured apart.  512 workgroups took 385 us where 256 took 374-379.
+// was not measured apart.  512 workgroups took 385 us where 256 took 374-379.  Rows of 7167 take 618 us, 4096 rows of 1024 f32
+// 31 us for 1001's 35: the unaligned and the f32 forms spill 6 to 26 registers a lane.
 // A workgroup walks the rows blockIdx.x * groups + group + i * gridDim.x * groups.  The next row is fetched
 // before the present one is reduced: the workgroup fills a CU, and without that nothing would be in flight while its
 // waves meet.  The vectors over the channels wait in LDS.  The sums over the rows stay in registers over the walk, two of
 // them, because d_w_post and the gradient of a gate per channel are both multiples of sum(dH u): each workgroup leaves one
 // row partial[2][gridDim.x][H] of sum(factor dH u) and sum(dn v), and norm_reduce_kernel adds those up in order.
 // WIDE (16 elements a lane): the sums are kept in the partial row itself, which the lane that owns the channel reads and
-// writes row by row, the vectors come from cache, and no row is fetched ahead.
+// writes row by row, the vectors are loaded again for every row, and no row is fetched ahead; 45 registers a lane spill, 231 to
+// 245 with unaligned rows.  8192 rows of 12288 bf16 take 1141 us (1.1 TB/s of the rows' bytes), of 16384 bf16 1487, f32 1922, of
+// 12289 bf16 2139: this form is right and no more.
 //
 // DN: there is a gradient of n.  Without one the residual is not read and nothing of h is formed, so an infinity or a NaN
-// in it (or in y, without a post norm) reaches no sum that it is not a term of.
+// in it (or in y, without a post norm) reaches no sum that it is not a term of: 16384 rows of 7168 bf16 with a post norm, 940
+// MB, 179 us (5.3 TB/s).
 struct NormGrad {
     const void *dh, *dn;                                     // either may be NULL
     const float *stats;
