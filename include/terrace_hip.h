@@ -531,11 +531,11 @@ TERRACE_API int terrace_w4_pack(const void *codes, const void *scales, const voi
 /* out[i] = W[e] x[i] for the rows i of expert e: x [P,K] and out [P,N] of dtype (BF16 or F16, the scales' type too),
  * rows in expert order, tokens_per_expert [n_experts] i64 (NULL with one expert: all rows are its rows).  swiglu != 0: N is even and out [P,N/2] =
  * silu(first half of the columns) * second half, taken before the one rounding.  Sums are fp32; infinities, NaN and
- * values up to the type's largest in x give what that sum of weight * x gives, some hundred times slower for their row.
+ * values up to the type's largest in x give what that sum of weight * x gives; a row with an infinity then takes some hundred times as long.
  * Rows past the last expert's are written as zeros.  Counts below 0 are taken as 0, and none reaches past row P.  x and the packed planes on 16 bytes.
  * Made for few rows per expert (every 16, 32 or 64 rows read the expert's weights once).  P is at most 2^30, and a launch
  * of 2^32 threads is refused: what reaches it is N / 32 * (experts that can hold a row + P / 16) >= 2^26 at 8 rows an expert
- * or fewer, N / 256 * (those experts + P / 64) >= 2^24 above. */
+ * or fewer, N / 256 * (those experts + P / 32) >= 2^24 above (P / 64 from 128 rows an expert on without zero points). */
 TERRACE_API int terrace_w4_linear(const void *x, int dtype, int64_t P, const int64_t *tokens_per_expert,
                                   const void *packed_codes, const void *packed_scales, const void *packed_zeros,
                                   int n_experts, int64_t N, int64_t K, int group, int swiglu, void *out,

@@ -333,8 +333,8 @@ def expert_linear_w4(rows, tokens_per_expert, weights: W4Weights, swiglu: bool =
 
     ``rows`` [P, K] of the weights' dtype in expert order and ``tokens_per_expert`` [E] int64 as :func:`expert_sort`,
     ``hopb_scatter`` and ``regroup`` (drop-less) give them; None with a single matrix: all rows are its rows.  Rows past
-    the last expert's give zero rows.  Infinities, NaN and very large values in a row give what the sum gives, for that
-    row, at some hundred times its time.  Made for serving, where an expert holds a few rows: the weights are read once per
+    the last expert's give zero rows.  Infinities, NaN and very large values in a row give what the sum gives; a row
+    with an infinity takes some hundred times as long.  Made for serving, where an expert holds a few rows: the weights are read once per
     16, 32 or 64 rows of an expert.  At most 2^30 rows; refused is also a launch of 2^32 threads, which takes some hundred
     thousand experts of a few rows each (``include/terrace_hip.h`` has the sum).  No gradients: a call that would need them
     raises."""
